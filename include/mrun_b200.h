@@ -566,6 +566,10 @@ int mrb_kv4_read(const void *pool, int64_t num_pages, int64_t hkv, int64_t head_
                  int64_t page_size, int64_t stride_page, int64_t stride_head, const int32_t *slots, int64_t tokens,
                  void *k_out, void *v_out, int out_dtype, int32_t *error_flag, void *stream);
 
+/* Of the workspaces of the two attentions below, the leading bytes that must be zero before the first
+ * use (their counters; the rest is partial results). */
+#define MRB_KV4_COUNTER_BYTES 8192
+
 /* Workspace bytes mrb_kv4_paged_attention needs for these sizes on the current device. */
 size_t mrb_kv4_paged_attention_workspace(int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim,
                                          int64_t max_total_tokens);
@@ -573,9 +577,9 @@ size_t mrb_kv4_paged_attention_workspace(int64_t rows, int64_t hq, int64_t hkv, 
 /* One-token grouped-query attention per row over the pool: row r attends to tokens
  * [0, row_len[r]) of block-table row row_seq[r] (NULL: r). q/out: bf16 [rows, hq, head_dim]. A
  * row without tokens gives zeros; tokens on a page outside [0, num_pages), or of a sequence outside
- * [0, num_seqs), are left out and set MRB_KV_UNMAPPED. max_total_tokens bounds row_len (longer rows are cut there). The workspace
- * must be zero-filled before its first use; calls leave it ready for the next one, and calls that
- * may overlap need their own. hq / hkv <= 16. */
+ * [0, num_seqs), are left out and set MRB_KV_UNMAPPED. max_total_tokens bounds row_len (longer rows are cut there). The counters
+ * of the workspace must be zeroed before its first use; calls leave it ready for the next one, and calls
+ * that may overlap need their own. hq / hkv <= 16. */
 int mrb_kv4_paged_attention(const void *q, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim, int64_t group,
                             const void *pool, int64_t num_pages, int64_t page_size, int64_t stride_page,
                             int64_t stride_head, const int32_t *block_table, int64_t num_seqs, int64_t block_table_stride,
@@ -592,8 +596,8 @@ int64_t mrb_kv4_paged_attention_timeouts(void);
  * [q_starts[r], q_starts[r + 1]) of q/out (bf16 [tokens, hq, head_dim]) are the last
  * q_starts[r + 1] - q_starts[r] of row r's row_len[r] tokens (q_starts[0] = 0, non-decreasing),
  * and each attends to the row's tokens up to its own. Query tokens from q_starts[rows] on are
- * not written. hq / hkv <= 16. `workspace` (_workspace bytes, 16-byte aligned, zeroed once) serves
- * one stream. */
+ * not written. hq / hkv <= 16. `workspace` (_workspace bytes, 16-byte aligned, its counters
+ * zeroed once) serves calls that do not overlap. */
 size_t mrb_kv4_prefill_attention_workspace(int64_t head_dim);
 int mrb_kv4_prefill_attention(const void *q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv,
                               int64_t head_dim, int64_t group, const void *pool, int64_t num_pages,

@@ -247,28 +247,37 @@ class DeviceScratch:
 class StreamScratch:
     """Zero-initialised workspace per (device, CUDA stream) for kernels whose workspace
     holds self-resetting counters: calls ordered on one stream may share it, calls on
-    different streams never do. While the current stream is being captured only an
-    existing buffer is handed out (None otherwise), so a CUDA graph never owns one."""
+    different streams never do. A captured call never gets it: the graph would keep an address
+    that a larger call on the stream later frees, and its replays on another stream would run
+    beside eager calls over the same counters. It gets memory of the graph's own instead."""
 
     def __init__(self) -> None:
         self._lock = threading.Lock()
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
 
-    def get(self, device: torch.device, nbytes: int) -> torch.Tensor | None:
+    def get(self, device: torch.device, nbytes: int, *, counters: int = 0) -> torch.Tensor | None:
+        """``counters``: the leading bytes that have to be zero. While the current stream is being
+        captured the buffer is the graph's, which clears those bytes at each replay; without a
+        number, all of it, and only where the stream has had a buffer (None otherwise)."""
         if nbytes <= 0:
             return None
         index = device.index if device.index is not None else torch.cuda.current_device()
         # the raw handle: building a Stream object costs as much as the rest of a small call
         key = (index, torch._C._cuda_getCurrentRawStream(index))
+        capturing = torch.cuda.is_current_stream_capturing()
         with self._lock:
             buf = self._buffers.get(key)
-            if buf is not None and buf.numel() >= nbytes:
+            have = buf is not None and buf.numel() >= nbytes
+            if not capturing:
+                if not have:
+                    buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
+                    self._buffers[key] = buf
                 return buf
-            if torch.cuda.is_current_stream_capturing():
-                return None
-            buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-            self._buffers[key] = buf
+        if counters:
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buf[:counters].zero_()
             return buf
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device) if have else None
 
 
 def exported_symbols() -> list[str]:

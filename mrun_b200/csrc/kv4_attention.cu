@@ -44,7 +44,7 @@ constexpr int KD_MAX_STAGES = 6;
 constexpr int KD_TILES = 2;  // tiles a unit: what a warp fetches, waits for and weighs in one go
 constexpr int KD_UNIT = KD_TILES * KV4_TILE;
 constexpr int KD_CHUNK = 64;       // parts of a group summed at a time
-constexpr int KD_COUNTERS = 8192;  // bytes of the workspace's counters, one a CTA
+constexpr int KD_COUNTERS = MRB_KV4_COUNTER_BYTES;  // of the workspace, one a CTA
 
 __device__ unsigned g_kv4_timeouts = 0;
 

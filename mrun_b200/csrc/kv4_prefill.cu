@@ -50,7 +50,7 @@ constexpr int KF_LEAST = 4;  // steps: no piece at a divided tile's ends is shor
 // Keys a CTA, before more CTAs divide tiles: joining many parts costs what it saves (8 tokens at 16000 x
 // 28/4 heads: 63 us, with 512 keys 87, with 2048 72).
 constexpr int KF_LEAST_KEYS = 1024;
-constexpr int KF_COUNTERS = 4096;  // bytes of the workspace's counters, one a CTA
+constexpr int KF_COUNTERS = MRB_KV4_COUNTER_BYTES;  // of the workspace, one a CTA
 
 __device__ unsigned g_kv4_prefill_timeouts = 0;
 

@@ -230,6 +230,7 @@ def kv4_read(pool: torch.Tensor, slots: torch.Tensor, *, group: int, head_dim: i
 
 _WORKSPACE = _lib.StreamScratch()
 _PREFILL_WORKSPACE = _lib.StreamScratch()
+_COUNTER_BYTES = 8192  # MRB_KV4_COUNTER_BYTES: what has to be zero of a workspace
 
 
 @lru_cache(maxsize=4096)
@@ -253,7 +254,8 @@ def kv4_paged_attention(
 ) -> torch.Tensor:
     """One query token per row, [rows, hq, d] bf16, over tokens ``[0, row_len[r])`` of sequence
     ``row_seq[r]`` (default r). ``max_total_tokens`` bounds the lengths. Rows without tokens give
-    zeros. The workspace, when given, must be zeroed once and serve one stream."""
+    zeros. The workspace, when given, must be zeroed once and serve one stream or one graph; by
+    default calls take their stream's, and captured calls one of the graph's own."""
     device = _lib.require_cuda(query, pool, block_table, row_len, what="4-bit paged attention")
     if query.dtype != torch.bfloat16:
         raise TypeError("4-bit paged attention runs on bf16 queries")
@@ -265,10 +267,7 @@ def kv4_paged_attention(
     rows, hq, d = q.shape
     need = kv4_paged_attention_workspace_bytes(rows, hq, pool.shape[1], d, max_total_tokens)
     if workspace is None:
-        if need:
-            workspace = _WORKSPACE.get(device, need)
-            if workspace is None:  # a capture without a workspace of its stream: one of the graph's own
-                workspace = torch.zeros(need, dtype=torch.uint8, device=device)
+        workspace = _WORKSPACE.get(device, need, counters=_COUNTER_BYTES)
     elif workspace.numel() < need:
         raise ValueError(f"workspace too small: {workspace.numel()} < {need} bytes")
     _lib.ops().kv4_paged_attention(q, pool, group, block_table, row_len, row_seq,
@@ -298,8 +297,7 @@ def kv4_prefill_attention(
 ) -> torch.Tensor:
     """Causal attention of ragged query blocks: ``query[q_starts[r]:q_starts[r + 1]]`` ([tokens, hq,
     d] bf16) are the last tokens of row r's ``row_len[r]`` cached ones (sequence ``row_seq[r]``,
-    default r), each attending up to itself. The workspace, when given, must be zeroed once and serve
-    one stream."""
+    default r), each attending up to itself. The workspace is as that of ``kv4_paged_attention``."""
     device = _lib.require_cuda(query, pool, block_table, q_starts, row_len, what="4-bit prefill attention")
     if query.dtype != torch.bfloat16:
         raise TypeError("4-bit prefill attention runs on bf16 queries")
@@ -310,9 +308,9 @@ def kv4_prefill_attention(
         out = torch.empty_like(q)
     need = kv4_prefill_attention_workspace_bytes(q.shape[2])
     if workspace is None:
-        workspace = _PREFILL_WORKSPACE.get(device, need)
-        if workspace is None:  # of a capture, when its stream has none (or the head_dim has no kernel)
-            workspace = torch.zeros(need, dtype=torch.uint8, device=device)
+        workspace = _PREFILL_WORKSPACE.get(device, need, counters=_COUNTER_BYTES)
+        if workspace is None:  # the head_dim has no kernel: the operator says so
+            workspace = torch.empty(0, dtype=torch.uint8, device=device)
     elif workspace.numel() < need:
         raise ValueError(f"workspace too small: {workspace.numel()} < {need} bytes")
     _lib.ops().kv4_prefill_attention(q, pool, group, block_table, q_starts, row_len, row_seq,
@@ -382,6 +380,9 @@ class PagedKV4Cache:
     def workspace_bytes(self, rows: int, num_heads: int, max_total_tokens: int) -> int:
         return kv4_paged_attention_workspace_bytes(rows, num_heads, self.kv_heads, self.head_dim, max_total_tokens)
 
+    def prefill_workspace_bytes(self) -> int:
+        return kv4_prefill_attention_workspace_bytes(self.head_dim)
+
     def attend(self, layer: int, query: torch.Tensor, row_len: torch.Tensor, *, max_total_tokens: int,
                row_seq: torch.Tensor | None = None, out: torch.Tensor | None = None,
                workspace: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
@@ -391,10 +392,10 @@ class PagedKV4Cache:
 
     def attend_prefill(self, layer: int, query: torch.Tensor, plan: KVStepPlan, *,
                        row_seq: torch.Tensor | None = None, scale: float | None = None,
-                       out: torch.Tensor | None = None) -> torch.Tensor:
+                       out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         return kv4_prefill_attention(query, self.pool[layer], group=self.group, block_table=self.block_table,
                                      q_starts=plan.q_starts, row_len=plan.row_len, row_seq=row_seq, scale=scale,
-                                     out=out, error_flag=self.error_flag)
+                                     out=out, workspace=workspace, error_flag=self.error_flag)
 
     def check_errors(self) -> None:
         """Raise on what the steps since the last call reported (synchronises)."""

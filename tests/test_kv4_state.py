@@ -1,0 +1,46 @@
+"""What the 4-bit cache and its operators keep between calls, without a GPU: default workspaces under
+capture and error bits."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import torch
+
+from mrun_b200 import _lib, paged_kv4
+
+
+def test_a_captured_call_gets_memory_of_the_graphs_own(monkeypatch):
+    """The stream's buffer is replaced by a larger one and serves eager calls: a graph must not hold it."""
+    capturing = [False]
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    dev = torch.device("cpu", 0)
+    for counters in (0, 64):
+        scratch = _lib.StreamScratch()
+        warm = scratch.get(dev, 1000, counters=counters)
+        warm.fill_(1)
+        capturing[0] = True
+        first, second = (scratch.get(dev, 1000, counters=counters) for _ in range(2))
+        capturing[0] = False
+        eager = scratch.get(dev, 1000, counters=counters)
+        assert eager.data_ptr() == warm.data_ptr()
+        assert len({first.data_ptr(), second.data_ptr(), warm.data_ptr()}) == 3
+        for buf in (first, second):
+            assert buf.numel() >= 1000 and not buf[:counters or 1000].any()
+
+
+def test_a_capture_on_a_stream_without_a_buffer(monkeypatch):
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 7, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    dev = torch.device("cpu", 0)
+    scratch = _lib.StreamScratch()
+    assert scratch.get(dev, 1000) is None  # callers that do without one
+    buf = scratch.get(dev, 1000, counters=64)
+    assert buf.numel() == 1000 and not buf[:64].any()
+    assert scratch.get(dev, 0, counters=64) is None
+
+
+def test_the_header_and_the_binding_agree_on_the_counters():
+    header = (Path(__file__).resolve().parents[1] / "include" / "mrun_b200.h").read_text()
+    assert int(re.search(r"#define MRB_KV4_COUNTER_BYTES (\d+)", header)[1]) == paged_kv4._COUNTER_BYTES

@@ -1,0 +1,78 @@
+"""What the 4-bit cache and its operators keep between calls, on the GPU."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_paged_kv4_gpu import _bf, _cache, _i32
+
+from oracle import kv4 as ok
+
+pytestmark = pytest.mark.gpu
+
+
+def _attention(which, cuda, seed, lengths, head_dim=128, hq=32, hkv=4):
+    """A call of one of the attentions over a cache of its own."""
+    from mrun_b200.paged_kv4 import kv4_paged_attention, kv4_prefill_attention
+
+    rng = np.random.default_rng(seed)
+    pool, table, _ = _cache(rng, lengths, hkv, head_dim, head_dim, 64, cuda)
+    q = _bf(ok.bf16(rng.standard_normal((len(lengths), hq, head_dim))), cuda)
+    common = dict(group=head_dim, block_table=table, row_len=_i32(lengths, cuda))
+    if which == "decode":
+        return lambda: kv4_paged_attention(q, pool, max_total_tokens=max(lengths), **common)
+    starts = _i32(list(range(len(lengths) + 1)), cuda)
+    return lambda: kv4_prefill_attention(q, pool, q_starts=starts, **common)
+
+
+@pytest.mark.parametrize("which", ["decode", "prefill"])
+def test_captured_calls_outlive_the_streams_workspace(which, cuda):
+    """Warm-up and two captures on one stream with default workspaces, a larger call on it, its old
+    memory taken by others: the graphs, replayed on two other streams at once, still give the same."""
+    small = _attention(which, cuda, 1, [4000], head_dim=64)
+    large = _attention(which, cuda, 2, [3000] * 32, head_dim=128)
+    want = small()
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        small()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(small())
+        graphs.append(graph)
+    with torch.cuda.stream(side):
+        large()
+    torch.cuda.synchronize()
+    taken = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=cuda) for _ in range(64)]
+    streams = [torch.cuda.Stream(cuda) for _ in graphs]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(side):
+            eager = small()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in (*outs, eager))
+    assert all((t == 255).all() for t in taken)
+
+
+def test_the_cache_passes_a_prefill_workspace_on(cuda):
+    from mrun_b200.paged_kv4 import PagedKV4Cache
+
+    c = PagedKV4Cache(num_layers=1, num_pages=40, kv_heads=2, head_dim=64, max_seqs=1, max_pages_per_seq=40, device=cuda)
+    plan = c.plan_step(_i32([600], cuda), max_tokens=600)
+    rng = np.random.default_rng(3)
+    rows = _bf(rng.standard_normal((600, 12 * 64)), cuda)
+    q = c.append(0, rows[:, 512:640], rows[:, 640:], plan, q_rows=rows[:, :512], num_heads=8)
+    ws = torch.zeros(c.prefill_workspace_bytes(), dtype=torch.uint8, device=cuda)
+    assert torch.equal(c.attend_prefill(0, q, plan, workspace=ws), c.attend_prefill(0, q, plan))
+    with pytest.raises(ValueError, match="workspace too small"):
+        c.attend_prefill(0, q, plan, workspace=ws[:100])
+    c.check_errors()
