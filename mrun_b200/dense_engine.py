@@ -533,12 +533,12 @@ class DenseDecoder:
         """Capture the decode step for ``rows`` rows (warm-up run first, outside the graph).
         The captured step advances in_ids/positions/row_len itself; call begin_decode again
         before replaying on new inputs."""
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))
         state = [self.in_ids, self.positions, self.row_len]
         if self.kv_bits == 4:  # taking pages leaves the free stack as it was but for its count
             state += [self.kv.lengths, self.kv.block_table, self.kv.free_count]
         saved = [x.clone() for x in state]
+        stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))  # the copies come before the warm-up
         with torch.cuda.stream(stream):
             self._decode_body(rows)  # warm-up (lazy attribute setup happens here)
         torch.cuda.current_stream(self.device).wait_stream(stream)

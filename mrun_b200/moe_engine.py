@@ -378,9 +378,9 @@ class MoeDecoder:
         captured: their copies are planned on the host from each layer's routes."""
         if self.streamed:
             raise RuntimeError("a decoder with host-tier experts steps eagerly (routes are read on the host)")
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))
         saved = (self.in_ids.clone(), self.positions.clone(), self.row_len.clone())
+        stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))  # the copies come before the warm-up
         with torch.cuda.stream(stream):
             self._decode_body(rows)  # warm-up outside the graph
         torch.cuda.current_stream(self.device).wait_stream(stream)

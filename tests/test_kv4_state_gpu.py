@@ -76,3 +76,31 @@ def test_the_cache_passes_a_prefill_workspace_on(cuda):
     with pytest.raises(ValueError, match="workspace too small"):
         c.attend_prefill(0, q, plan, workspace=ws[:100])
     c.check_errors()
+
+
+def _dense(cuda, **kw):
+    from mrun_b200.dense_engine import DenseConfig, DenseDecoder, DenseWeights
+
+    cfg = DenseConfig(num_layers=2, hidden=256, heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=1000)
+    args = dict(max_batch=2, max_seq_len=192, device=cuda, max_prefill_tokens=192, kv_bits=4) | kw
+    return cfg, DenseDecoder(DenseWeights.synthetic(cfg, cuda, seed=5), **args)
+
+
+def test_capture_while_the_stream_is_busy(cuda):
+    """The state that a capture's warm-up changes is copied before the warm-up runs, whatever is queued
+    on the stream (here work of tens of milliseconds, with no word to the host in between)."""
+    cfg, dec = _dense(cuda)
+    ids = torch.arange(128) % cfg.vocab
+    firsts = dec.prefill_batch([0, 1], [ids[:64], ids[:63]])  # the next token of row 0 takes a page
+    dec.begin_decode(2, firsts, [64, 63])
+    table, free = dec.kv.block_table.clone(), dec.kv.free_count.item()
+    a = torch.randn(8192, 8192, device=cuda, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    for _ in range(40):
+        a = torch.mm(a, a)
+    dec.capture(2)
+    assert dec.kv.lengths.tolist() == [64, 63] and dec.kv.free_count.item() == free
+    assert torch.equal(dec.kv.block_table, table)
+    assert dec.positions[:2].tolist() == [64, 63] and dec.row_len[:2].tolist() == [65, 64]
+    assert torch.equal(dec.in_ids[:2], firsts)
+    dec.check_errors()
