@@ -516,6 +516,7 @@ enum {
   MRB_KV_POOL_EMPTY = 8,   /* not enough free pages */
   MRB_KV_BAD_SLOT = 16,    /* a slot (other than -1) or position out of range: the token is skipped */
   MRB_KV_UNMAPPED = 32,    /* attention met an unmapped page: its tokens are left out */
+  MRB_KV_TIMEOUT = 64,     /* a bounded wait of an attention ran out: its output is void */
 };
 
 /* The page plan of one step, built on the device. Request r appends new_tokens[r] >= 0 tokens to

@@ -402,8 +402,10 @@ kv4_decode_kernel(const __grid_constant__ Kv4DecodeArgs a) {
     }
 
     for (; k < n && lo + warp + k * W < seg_end; ++k) {
-      if (!mbar_try_wait(bar + stage, phase) && !mbar_wait_bounded(bar + stage, phase) && lane == 0)
+      if (!mbar_try_wait(bar + stage, phase) && !mbar_wait_bounded(bar + stage, phase) && lane == 0) {
         atomicAdd(&g_kv4_timeouts, 1u);
+        if (a.error_flag) atomicOr(a.error_flag, MRB_KV_TIMEOUT);
+      }
       __syncwarp();
       const int lim = lim_of[stage];
       const unsigned char* st = ring + stage * STAGE;

@@ -1063,6 +1063,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
       for (int i = 0; i < 2; ++i) mbar_wait_bounded(&sh.o_full[i], (turns - 1) & 1);
   }
   __syncthreads();
+  if (tid == 0 && sh.dead && a.error_flag) atomicOr(a.error_flag, MRB_KV_TIMEOUT);
   if (warp == (KF_SOFTMAX + KF_FILL) / 32) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

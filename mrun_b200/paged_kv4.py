@@ -35,6 +35,7 @@ KV_TOKENS_FULL = 4
 KV_POOL_EMPTY = 8
 KV_BAD_SLOT = 16
 KV_UNMAPPED = 32
+KV_TIMEOUT = 64
 
 _ERRORS = {
     KV_BAD_REQUEST: "a sequence out of range or twice in a step, a negative count, or a damaged page list",
@@ -43,6 +44,7 @@ _ERRORS = {
     KV_POOL_EMPTY: "the paged KV pool is exhausted",
     KV_BAD_SLOT: "an append saw a slot or position out of range",
     KV_UNMAPPED: "attention met an unmapped page",
+    KV_TIMEOUT: "a wait inside an attention kernel ran out, its outputs are void",
 }
 
 

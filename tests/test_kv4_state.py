@@ -5,6 +5,7 @@ from __future__ import annotations
 import re
 from pathlib import Path
 
+import pytest
 import torch
 
 from mrun_b200 import _lib, paged_kv4
@@ -44,3 +45,23 @@ def test_a_capture_on_a_stream_without_a_buffer(monkeypatch):
 def test_the_header_and_the_binding_agree_on_the_counters():
     header = (Path(__file__).resolve().parents[1] / "include" / "mrun_b200.h").read_text()
     assert int(re.search(r"#define MRB_KV4_COUNTER_BYTES (\d+)", header)[1]) == paged_kv4._COUNTER_BYTES
+
+
+def _header() -> str:
+    return (Path(__file__).resolve().parents[1] / "include" / "mrun_b200.h").read_text()
+
+
+def test_every_error_bit_has_a_name_and_a_text():
+    bits = {name: int(value) for name, value in re.findall(r"MRB_(KV_\w+) = (\d+),", _header())}
+    assert bits and all(getattr(paged_kv4, name) == value for name, value in bits.items())
+    assert sorted(paged_kv4._ERRORS) == sorted(bits.values())
+
+
+def test_a_wait_that_ran_out_is_an_error():
+    """A kernel whose bounded wait ran out has written what is no result: the cache says so."""
+    cache = paged_kv4.PagedKV4Cache(num_layers=1, num_pages=2, kv_heads=1, head_dim=64, max_seqs=1,
+                                    max_pages_per_seq=2, device=torch.device("cpu"))
+    cache.error_flag.fill_(paged_kv4.KV_TIMEOUT)
+    with pytest.raises(RuntimeError, match="ran out"):
+        cache.check_errors()
+    cache.check_errors()
