@@ -517,6 +517,7 @@ enum {
   MRB_KV_BAD_SLOT = 16,    /* a slot (other than -1) or position out of range: the token is skipped */
   MRB_KV_UNMAPPED = 32,    /* attention met an unmapped page: its tokens are left out */
   MRB_KV_TIMEOUT = 64,     /* a bounded wait of an attention ran out: its output is void */
+  MRB_KV_TOO_LONG = 128,   /* a row longer than max_total_tokens or its block-table row was cut there */
 };
 
 /* The page plan of one step, built on the device. Request r appends new_tokens[r] >= 0 tokens to
@@ -578,7 +579,8 @@ size_t mrb_kv4_paged_attention_workspace(int64_t rows, int64_t hq, int64_t hkv, 
 /* One-token grouped-query attention per row over the pool: row r attends to tokens
  * [0, row_len[r]) of block-table row row_seq[r] (NULL: r). q/out: bf16 [rows, hq, head_dim]. A
  * row without tokens gives zeros; tokens on a page outside [0, num_pages), or of a sequence outside
- * [0, num_seqs), are left out and set MRB_KV_UNMAPPED. max_total_tokens bounds row_len (longer rows are cut there). The counters
+ * [0, num_seqs), are left out and set MRB_KV_UNMAPPED. max_total_tokens bounds row_len (longer rows are
+ * cut there or at their block-table row's end, MRB_KV_TOO_LONG). The counters
  * of the workspace must be zeroed before its first use; calls leave it ready for the next one, and calls
  * that may overlap need their own. hq / hkv <= 16. */
 int mrb_kv4_paged_attention(const void *q, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim, int64_t group,
@@ -596,7 +598,8 @@ int64_t mrb_kv4_paged_attention_timeouts(void);
 /* Causal attention of ragged query blocks whose keys and values are in the pool: tokens
  * [q_starts[r], q_starts[r + 1]) of q/out (bf16 [tokens, hq, head_dim]) are the last
  * q_starts[r + 1] - q_starts[r] of row r's row_len[r] tokens (q_starts[0] = 0, non-decreasing),
- * and each attends to the row's tokens up to its own. Query tokens from q_starts[rows] on are
+ * and each attends to the row's tokens up to its own, as far as its block-table row goes
+ * (MRB_KV_TOO_LONG). Query tokens from q_starts[rows] on are
  * not written. hq / hkv <= 16. `workspace` (_workspace bytes, 16-byte aligned, its counters
  * zeroed once) serves calls that do not overlap. */
 size_t mrb_kv4_prefill_attention_workspace(int64_t head_dim);

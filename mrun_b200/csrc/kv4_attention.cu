@@ -137,7 +137,8 @@ __device__ __forceinline__ int kd_prefix(const Kv4DecodeArgs& a, int extra, int*
   const int per = (a.rows + threads - 1) / threads, r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
   int mine = 0;
   for (int r = r0; r < r1; ++r) {
-    const int len = min(a.row_len[a.row0 + r], a.cap);
+    const int all = a.row_len[a.row0 + r], len = min(all, a.cap);
+    if (all > a.cap && blockIdx.x == 0 && a.error_flag) atomicOr(a.error_flag, MRB_KV_TOO_LONG);
     pre[r] = len > 0 ? ((len + KD_UNIT - 1) / KD_UNIT + extra) * a.pool.hkv : 0;
     mine += pre[r];
   }

@@ -292,6 +292,7 @@ __device__ __noinline__ void kf_plan(const Kv4PrefillArgs& a, KfShared& sh, int 
     int64_t work = 0, tiles = 0;
     for (int r = lane; r < a.rows; r += 32) {
       const KfBlock b = kf_block(a, r, span);
+      if (b.count > 0 && a.row_len[r] > a.cap && cta == 0 && a.error_flag) atomicOr(a.error_flag, MRB_KV_TOO_LONG);
       work += kf_length(b, span, b.tiles);
       tiles += b.tiles;
     }

@@ -36,6 +36,7 @@ KV_POOL_EMPTY = 8
 KV_BAD_SLOT = 16
 KV_UNMAPPED = 32
 KV_TIMEOUT = 64
+KV_TOO_LONG = 128
 
 _ERRORS = {
     KV_BAD_REQUEST: "a sequence out of range or twice in a step, a negative count, or a damaged page list",
@@ -45,6 +46,7 @@ _ERRORS = {
     KV_BAD_SLOT: "an append saw a slot or position out of range",
     KV_UNMAPPED: "attention met an unmapped page",
     KV_TIMEOUT: "a wait inside an attention kernel ran out, its outputs are void",
+    KV_TOO_LONG: "attention met a row longer than max_total_tokens or than its block-table row",
 }
 
 
@@ -255,7 +257,8 @@ def kv4_paged_attention(
     error_flag: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """One query token per row, [rows, hq, d] bf16, over tokens ``[0, row_len[r])`` of sequence
-    ``row_seq[r]`` (default r). ``max_total_tokens`` bounds the lengths. Rows without tokens give
+    ``row_seq[r]`` (default r). ``max_total_tokens`` bounds the lengths (``KV_TOO_LONG``
+    is set where one is cut). Rows without tokens give
     zeros. The workspace, when given, must be zeroed once and serve one stream or one graph; by
     default calls take their stream's, and captured calls one of the graph's own."""
     device = _lib.require_cuda(query, pool, block_table, row_len, what="4-bit paged attention")
@@ -407,7 +410,7 @@ class PagedKV4Cache:
             text = "; ".join(message for bit, message in _ERRORS.items() if bits & bit)
             if bits & KV_POOL_EMPTY:
                 raise MemoryError(text)
-            if bits & (KV_TABLE_FULL | KV_TOKENS_FULL):
+            if bits & (KV_TABLE_FULL | KV_TOKENS_FULL | KV_TOO_LONG):
                 raise OverflowError(text)
             raise RuntimeError(text)
 

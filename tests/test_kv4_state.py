@@ -65,3 +65,11 @@ def test_a_wait_that_ran_out_is_an_error():
     with pytest.raises(RuntimeError, match="ran out"):
         cache.check_errors()
     cache.check_errors()
+
+
+def test_a_row_that_was_cut_is_an_error():
+    cache = paged_kv4.PagedKV4Cache(num_layers=1, num_pages=2, kv_heads=1, head_dim=64, max_seqs=1,
+                                    max_pages_per_seq=2, device=torch.device("cpu"))
+    cache.error_flag.fill_(paged_kv4.KV_TOO_LONG)
+    with pytest.raises(OverflowError, match="longer than"):
+        cache.check_errors()

@@ -104,3 +104,28 @@ def test_capture_while_the_stream_is_busy(cuda):
     assert dec.positions[:2].tolist() == [64, 63] and dec.row_len[:2].tolist() == [65, 64]
     assert torch.equal(dec.in_ids[:2], firsts)
     dec.check_errors()
+
+
+def test_rows_that_are_cut_are_reported(cuda):
+    """A row longer than max_total_tokens, or than its block-table row, is cut there, and says so."""
+    from mrun_b200.paged_kv4 import KV_TOO_LONG, kv4_paged_attention, kv4_prefill_attention
+
+    from test_paged_kv4_gpu import _check
+
+    rng = np.random.default_rng(5)
+    lengths = [40, 64, 100]
+    pool, table, cache = _cache(rng, lengths, 2, 64, 32, 16, cuda)
+    q = ok.bf16(rng.standard_normal((3, 4, 64)))
+    ln, starts = _i32(lengths, cuda), _i32([0, 1, 2, 3], cuda)
+    narrow = table[:, :4].contiguous()
+    for table_, most, cut in ((table, 100, 100), (table, 64, 64), (table, 0, 0), (narrow, 100, 64)):
+        for prefill in (False, True):
+            if prefill and table_ is table:
+                continue
+            flag = torch.zeros(1, dtype=torch.int32, device=cuda)
+            common = dict(group=32, block_table=table_, row_len=ln, error_flag=flag)
+            got = (kv4_prefill_attention(_bf(q, cuda), pool, q_starts=starts, **common) if prefill else
+                   kv4_paged_attention(_bf(q, cuda), pool, max_total_tokens=most, **common))
+            assert flag.item() == (KV_TOO_LONG if cut < 100 else 0)
+            for r in range(3):
+                _check(got[r], *ok.attend(q[r], cache[r], min(lengths[r], cut), 64 ** -0.5))
