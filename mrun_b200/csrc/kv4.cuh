@@ -76,7 +76,8 @@ inline int kv4_check_attention(const char* what, const void* q, int64_t tokens, 
       block_table_stride < max_pages_per_seq)
     return fail(MRB_ERR_ARG, "%s: bad sizes", what);
   if (hq / hkv > KV4_MAX_GROUP) return fail(MRB_ERR_UNSUPPORTED, "%s: at most 16 query heads a KV head", what);
-  if (max_pages_per_seq > INT32_MAX / page_size || hkv > 65535 || tokens > INT32_MAX || rows > INT32_MAX)
+  // (the kernels round positions up to their steps of 128 tokens)
+  if (max_pages_per_seq > (INT32_MAX - 128) / page_size || hkv > 65535 || tokens > INT32_MAX || rows > INT32_MAX)
     return fail(MRB_ERR_UNSUPPORTED, "%s: positions and rows must be numbered in 32 bits", what);
   if (!isfinite(scale)) return fail(MRB_ERR_ARG, "%s: scale must be finite", what);
   if (tokens == 0 || rows == 0) return MRB_OK;

@@ -276,7 +276,7 @@ __device__ __forceinline__ KfBlock kf_block(const Kv4PrefillArgs& a, int r, int 
   b.count = a.q_starts[r + 1] - b.q0;
   if (b.q0 < 0 || (int64_t)b.q0 + b.count > a.tokens) b.count = 0;  // not a block of these queries
   b.tiles = b.count > 0 ? (b.count + span - 1) / span : 0;
-  b.base = max(0, min(a.row_len[r], a.cap) - b.count);
+  b.base = max(0, min(max(a.row_len[r], 0), a.cap) - b.count);
   return b;
 }
 // the length of a block's first t < tiles tiles of one head, and of all
@@ -361,7 +361,7 @@ __device__ __noinline__ void kf_plan(const Kv4PrefillArgs& a, KfShared& sh, int 
   if (row < a.rows) {
     const int64_t begin = cuts.at(cta), end = cuts.at(cta + 1);
     KfBlock b = kf_block(a, row, span);
-    int len = a.row_len[row];
+    int len = max(a.row_len[row], 0);
     while (true) {
       const int64_t before = kf_length(b, span, t), length = kf_length(b, span, t + 1) - before;
       const int64_t from = at + before * hkv + head * length;
@@ -405,7 +405,7 @@ __device__ __noinline__ void kf_plan(const Kv4PrefillArgs& a, KfShared& sh, int 
       t = 0;
       if (++row >= a.rows) break;
       b = kf_block(a, row, span);
-      len = a.row_len[row];
+      len = max(a.row_len[row], 0);
     }
   }
   __syncwarp();

@@ -10,6 +10,8 @@ import torch
 
 from mrun_b200 import _lib, paged_kv4
 
+from test_paged_kv4 import _decode, _prefill
+
 
 def test_a_captured_call_gets_memory_of_the_graphs_own(monkeypatch):
     """The stream's buffer is replaced by a larger one and serves eager calls: a graph must not hold it."""
@@ -73,3 +75,10 @@ def test_a_row_that_was_cut_is_an_error():
     cache.error_flag.fill_(paged_kv4.KV_TOO_LONG)
     with pytest.raises(OverflowError, match="longer than"):
         cache.check_errors()
+
+
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_positions_that_cannot_be_rounded_up_are_refused(call):
+    """2^31 - 16 tokens a row: their last step's end is past 32 bits."""
+    pages = (2 ** 31 - 1) // 16
+    assert call(_lib.load(), per=pages, stride=pages) == _lib.MRB_ERR_UNSUPPORTED

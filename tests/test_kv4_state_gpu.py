@@ -129,3 +129,16 @@ def test_rows_that_are_cut_are_reported(cuda):
             assert flag.item() == (KV_TOO_LONG if cut < 100 else 0)
             for r in range(3):
                 _check(got[r], *ok.attend(q[r], cache[r], min(lengths[r], cut), 64 ** -0.5))
+
+
+def test_negative_lengths_are_none(cuda):
+    from mrun_b200.paged_kv4 import kv4_paged_attention, kv4_prefill_attention
+
+    rng = np.random.default_rng(6)
+    pool, table, _ = _cache(rng, [40] * 4, 2, 64, 32, 16, cuda)
+    q = _bf(ok.bf16(rng.standard_normal((4, 4, 64))), cuda)
+    common = dict(group=32, block_table=table, row_len=_i32([-2 ** 31, -1, 0, 40], cuda))
+    a = kv4_paged_attention(q, pool, max_total_tokens=40, **common)
+    b = kv4_prefill_attention(q, pool, q_starts=_i32([0, 1, 2, 3, 4], cuda), **common)
+    for out in (a, b):
+        assert not out[:3].any() and out[3].any()
