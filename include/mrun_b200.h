@@ -610,6 +610,15 @@ int mrb_kv4_prefill_attention(const void *q, int64_t tokens, int64_t rows, int64
                               int64_t max_pages_per_seq, const int32_t *q_starts, const int32_t *row_seq,
                               const int32_t *row_len, float scale, void *out, void *workspace,
                               size_t workspace_bytes, int32_t *error_flag, void *stream);
+/* The same, but query tokens from q_starts[rows] on (all, after a plan that did not fit) give zeros
+ * (rows = 0 still does nothing). */
+int mrb_kv4_prefill_attention_all(const void *q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv,
+                                  int64_t head_dim, int64_t group, const void *pool, int64_t num_pages,
+                                  int64_t page_size, int64_t stride_page, int64_t stride_head,
+                                  const int32_t *block_table, int64_t num_seqs, int64_t block_table_stride,
+                                  int64_t max_pages_per_seq, const int32_t *q_starts, const int32_t *row_seq,
+                                  const int32_t *row_len, float scale, void *out, void *workspace,
+                                  size_t workspace_bytes, int32_t *error_flag, void *stream);
 
 /* As mrb_kv4_paged_attention_timeouts, of mrb_kv4_prefill_attention. */
 int64_t mrb_kv4_prefill_attention_timeouts(void);

@@ -109,6 +109,8 @@ SIGNATURES: dict[str, list] = {
     "mrb_kv4_prefill_attention_workspace": [_I64],
     "mrb_kv4_prefill_attention": [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64,
                                   _P, _P, _P, c_float, _P, _P, c_size_t, _P, _P],
+    "mrb_kv4_prefill_attention_all": [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64,
+                                      _I64, _P, _P, _P, c_float, _P, _P, c_size_t, _P, _P],
 }
 _RESTYPES = {"mrb_last_error": ctypes.c_char_p, "mrb_abi_version": c_int, "mrb_paged_attention_workspace": c_size_t,
              "mrb_paged_attention_static_capacity": c_size_t, "mrb_qrow_workspace": c_size_t,

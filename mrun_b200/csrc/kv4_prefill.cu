@@ -64,6 +64,7 @@ struct Kv4PrefillArgs {
   float* part;
   int64_t tokens, bt_stride, num_seqs;
   int rows, hq, cap;
+  bool zero_rest;  // query tokens of no block give zeros
   uint32_t page_magic, group_magic;  // of a page's 16-token blocks and of a group, as kf_divide takes them
   uint32_t q_and, q_xor;  // applied to query pairs: a negative or zero scale
   float scale2;           // |softmax scale| log2(e)
@@ -1007,10 +1008,18 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
       if (i == 1) umma_commit(&sh.k_empty[at & 1]);
     };
     int walked = 0, turns = 0;
-    bool more;
+    bool more, idle = warp != (KF_SOFTMAX + KF_FILL) / 32 && a.zero_rest;
     do {
       kf_all_sync();
       more = sh.more;
+      if (idle) {  // the warps that issue nothing write the zeros
+        constexpr int FIRST = KF_SOFTMAX + KF_FILL + 32, COUNT = KF_THREADS - FIRST;
+        const int64_t row = (int64_t)a.hq * (D / 8), end = a.tokens * row;
+        const int from = max(0, a.q_starts[a.rows]);
+        for (int64_t x = from * row + blockIdx.x * COUNT + tid - FIRST; x < end; x += gridDim.x * COUNT)
+          reinterpret_cast<uint4*>(a.out)[x] = make_uint4(0u, 0u, 0u, 0u);
+        idle = false;
+      }
       const int pieces = warp == (KF_SOFTMAX + KF_FILL) / 32 ? sh.pieces : 0;
 #pragma unroll 1
       for (int n = 0; n < pieces; ++n) {
@@ -1099,14 +1108,12 @@ extern "C" size_t mrb_kv4_prefill_attention_workspace(int64_t head_dim) {
   return head_dim == 64 || head_dim == 128 ? mrb::kf_workspace(head_dim) : 0;
 }
 
-extern "C" int mrb_kv4_prefill_attention(const void* q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv,
-                                         int64_t head_dim, int64_t group, const void* pool, int64_t num_pages,
-                                         int64_t page_size, int64_t stride_page, int64_t stride_head,
-                                         const int32_t* block_table, int64_t num_seqs, int64_t block_table_stride,
-                                         int64_t max_pages_per_seq, const int32_t* q_starts, const int32_t* row_seq,
-                                         const int32_t* row_len, float scale, void* out, void* workspace,
-                                         size_t workspace_bytes, int32_t* error_flag, void* stream) {
-  using namespace mrb;
+namespace mrb {
+static int prefill(const void* q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv, int64_t head_dim, int64_t group,
+                   const void* pool, int64_t num_pages, int64_t page_size, int64_t stride_page, int64_t stride_head,
+                   const int32_t* block_table, int64_t num_seqs, int64_t block_table_stride, int64_t max_pages_per_seq,
+                   const int32_t* q_starts, const int32_t* row_seq, const int32_t* row_len, float scale, void* out,
+                   bool zero_rest, void* workspace, size_t workspace_bytes, int32_t* error_flag, void* stream) {
   const char* what = "kv4_prefill_attention";
   Kv4PrefillArgs a = {};
   const int rc = kv4_check_attention(what, q, tokens, rows, hq, hkv, head_dim, group, pool, num_pages, page_size,
@@ -1131,6 +1138,7 @@ extern "C" int mrb_kv4_prefill_attention(const void* q, int64_t tokens, int64_t 
   a.counters = (unsigned*)workspace;
   a.part = (float*)((char*)workspace + KF_COUNTERS);
   a.tokens = tokens;
+  a.zero_rest = zero_rest;
   a.bt_stride = block_table_stride;
   a.num_seqs = num_seqs;
   a.rows = (int)rows;
@@ -1148,4 +1156,30 @@ extern "C" int mrb_kv4_prefill_attention(const void* q, int64_t tokens, int64_t 
   if (group == 32) return launch_prefill<128, 32>(a, s);
   if (group == 64) return launch_prefill<128, 64>(a, s);
   return launch_prefill<128, 128>(a, s);
+}
+}  // namespace mrb
+
+extern "C" int mrb_kv4_prefill_attention(const void* q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv,
+                                         int64_t head_dim, int64_t group, const void* pool, int64_t num_pages,
+                                         int64_t page_size, int64_t stride_page, int64_t stride_head,
+                                         const int32_t* block_table, int64_t num_seqs, int64_t block_table_stride,
+                                         int64_t max_pages_per_seq, const int32_t* q_starts, const int32_t* row_seq,
+                                         const int32_t* row_len, float scale, void* out, void* workspace,
+                                         size_t workspace_bytes, int32_t* error_flag, void* stream) {
+  return mrb::prefill(q, tokens, rows, hq, hkv, head_dim, group, pool, num_pages, page_size, stride_page, stride_head,
+                      block_table, num_seqs, block_table_stride, max_pages_per_seq, q_starts, row_seq, row_len, scale,
+                      out, false, workspace, workspace_bytes, error_flag, stream);
+}
+
+extern "C" int mrb_kv4_prefill_attention_all(const void* q, int64_t tokens, int64_t rows, int64_t hq, int64_t hkv,
+                                             int64_t head_dim, int64_t group, const void* pool, int64_t num_pages,
+                                             int64_t page_size, int64_t stride_page, int64_t stride_head,
+                                             const int32_t* block_table, int64_t num_seqs, int64_t block_table_stride,
+                                             int64_t max_pages_per_seq, const int32_t* q_starts,
+                                             const int32_t* row_seq, const int32_t* row_len, float scale, void* out,
+                                             void* workspace, size_t workspace_bytes, int32_t* error_flag,
+                                             void* stream) {
+  return mrb::prefill(q, tokens, rows, hq, hkv, head_dim, group, pool, num_pages, page_size, stride_page, stride_head,
+                      block_table, num_seqs, block_table_stride, max_pages_per_seq, q_starts, row_seq, row_len, scale,
+                      out, true, workspace, workspace_bytes, error_flag, stream);
 }

@@ -438,7 +438,7 @@ void kv4_paged_attention(const at::Tensor& q, const at::Tensor& pool, int64_t gr
 void kv4_prefill_attention(const at::Tensor& q, const at::Tensor& pool, int64_t group, const at::Tensor& block_table,
                            const at::Tensor& q_starts, const at::Tensor& row_len,
                            const std::optional<at::Tensor>& row_seq, double scale, at::Tensor& out,
-                           const at::Tensor& workspace, const std::optional<at::Tensor>& error_flag) {
+                           const at::Tensor& workspace, const std::optional<at::Tensor>& error_flag, bool zero_rest) {
   const char* what = "kv4_prefill_attention";
   const c10::cuda::CUDAGuard guard(pool.device());
   const Pool p = pool_of(pool, group);
@@ -453,7 +453,8 @@ void kv4_prefill_attention(const at::Tensor& q, const at::Tensor& pool, int64_t 
   TORCH_CHECK_VALUE(q_starts.numel() == rows + 1, what, ": q_starts must hold one entry a row and the end");
   TORCH_CHECK_VALUE((row_seq.has_value() && row_seq->defined()) || rows <= block_table.size(0), what,
                     ": more rows than sequences");
-  check_status(mrb_kv4_prefill_attention(
+  const auto run = zero_rest ? &mrb_kv4_prefill_attention_all : &mrb_kv4_prefill_attention;
+  check_status(run(
                    q.data_ptr(), q.size(0), rows, hq, p.hkv, p.head_dim, group, pool.data_ptr(), p.pages, p.page_size,
                    p.stride_page, p.stride_head, block_table.data_ptr<int32_t>(), block_table.size(0),
                    table_stride(block_table), block_table.size(1), q_starts.data_ptr<int32_t>(), opt_i32(row_seq, pool, rows, "row_seq", what),
@@ -492,8 +493,8 @@ TORCH_LIBRARY(mrun_b200, m) {
   m.def("kv4_paged_attention(Tensor q, Tensor pool, int group, Tensor block_table, Tensor row_len, Tensor? row_seq, "
         "float scale, int max_total_tokens, Tensor(a!) out, Tensor(b!)? workspace, Tensor(c!)? error_flag) -> ()");
   m.def("kv4_prefill_attention(Tensor q, Tensor pool, int group, Tensor block_table, Tensor q_starts, "
-        "Tensor row_len, Tensor? row_seq, float scale, Tensor(a!) out, Tensor(c!) workspace, Tensor(b!)? error_flag) "
-        "-> ()");
+        "Tensor row_len, Tensor? row_seq, float scale, Tensor(a!) out, Tensor(c!) workspace, Tensor(b!)? error_flag, "
+        "bool zero_rest=False) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(mrun_b200, CUDA, m) {

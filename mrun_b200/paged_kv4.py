@@ -302,15 +302,18 @@ def kv4_prefill_attention(
 ) -> torch.Tensor:
     """Causal attention of ragged query blocks: ``query[q_starts[r]:q_starts[r + 1]]`` ([tokens, hq,
     d] bf16) are the last tokens of row r's ``row_len[r]`` cached ones (sequence ``row_seq[r]``,
-    default r), each attending up to itself. The workspace is as that of ``kv4_paged_attention``."""
+    default r), each attending up to itself. Tokens of no block (from ``q_starts[rows]`` on: padding, or
+    all of them after a plan that did not fit) give zeros; in a given ``out`` they stay as they are. The
+    workspace is as that of ``kv4_paged_attention``."""
     device = _lib.require_cuda(query, pool, block_table, q_starts, row_len, what="4-bit prefill attention")
     if query.dtype != torch.bfloat16:
         raise TypeError("4-bit prefill attention runs on bf16 queries")
     if query.ndim != 3 or pool.ndim != 4:
         raise ValueError("query must be [tokens, heads, head_dim] and the pool [pages, kv_heads, tiles, block_bytes]")
     q = query.contiguous()
+    zero_rest = out is None
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q) if row_len.numel() else torch.zeros_like(q)
     need = kv4_prefill_attention_workspace_bytes(q.shape[2])
     if workspace is None:
         workspace = _PREFILL_WORKSPACE.get(device, need, counters=_COUNTER_BYTES)
@@ -320,7 +323,7 @@ def kv4_prefill_attention(
         raise ValueError(f"workspace too small: {workspace.numel()} < {need} bytes")
     _lib.ops().kv4_prefill_attention(q, pool, group, block_table, q_starts, row_len, row_seq,
                                      1.0 / math.sqrt(q.shape[2]) if scale is None else scale, out, workspace,
-                                     error_flag)
+                                     error_flag, zero_rest)
     return out
 
 

@@ -142,3 +142,35 @@ def test_negative_lengths_are_none(cuda):
     b = kv4_prefill_attention(q, pool, q_starts=_i32([0, 1, 2, 3, 4], cuda), **common)
     for out in (a, b):
         assert not out[:3].any() and out[3].any()
+
+
+def test_queries_of_no_block_give_zeros(cuda):
+    """Padding past the last block, every query after a plan that did not fit, and a call without rows."""
+    from mrun_b200.paged_kv4 import KVStepPlan, PagedKV4Cache, kv4_prefill_attention
+
+    rng = np.random.default_rng(7)
+    for head_dim, tokens in ((64, 40), (128, 3000)):
+        c = PagedKV4Cache(num_layers=1, num_pages=4, kv_heads=2, head_dim=head_dim, max_seqs=2, max_pages_per_seq=2,
+                          device=cuda)
+        q = _bf(rng.standard_normal((tokens, 6, head_dim)), cuda)
+        rows = _bf(rng.standard_normal((tokens, 4 * head_dim)), cuda)
+        plan = KVStepPlan.empty(2, tokens, cuda)
+        for new, fits in (([9, 21], True), ([0, 0], True), ([9, 40], False)):
+            c.plan_step(_i32(new, cuda), max_tokens=tokens, out=plan)
+            c.append(0, rows[:, :2 * head_dim], rows[:, 2 * head_dim:], plan)
+            used = sum(new) if fits else 0
+            poison = torch.full_like(q, float("nan"))  # what the outputs' memory held before
+            del poison
+            got = c.attend_prefill(0, q, plan)
+            assert got[:used].any(-1).all() and not got[used:].any()
+            kept = c.attend_prefill(0, q, plan, out=torch.full_like(q, 7))
+            assert torch.equal(kept[:used], got[:used]) and (kept[used:] == 7).all()
+            if fits:
+                c.check_errors()
+            c.release(_i32([0, 1], cuda))
+        none = _i32([], cuda)
+        poison = torch.full_like(q, float("nan"))
+        del poison
+        got = kv4_prefill_attention(q, c.pool[0], group=head_dim, block_table=c.block_table, q_starts=_i32([0], cuda),
+                                    row_len=none)
+        assert not got.any()
