@@ -562,6 +562,15 @@ int mrb_rope_kv4_append(const void *q_in, const void *k_in, const void *v_in, in
                         int64_t num_pages, int64_t page_size, int64_t stride_page, int64_t stride_head,
                         int32_t *error_flag, void *stream);
 
+/* The same with a row stride for queries (0 without them) and one for keys. */
+int mrb_rope_kv4_append_strided(const void *q_in, const void *k_in, const void *v_in, int64_t q_row_stride,
+                                int64_t k_row_stride, int64_t v_row_stride, int64_t tokens, int64_t hq, int64_t hkv,
+                                int64_t head_dim, int64_t group, const int32_t *positions, const int32_t *slots,
+                                const float *rope_cos, const float *rope_sin, int64_t rope_len, int64_t rotary_dim,
+                                int interleaved, const void *q_norm, const void *k_norm, float norm_eps, void *q_out,
+                                void *pool, int64_t num_pages, int64_t page_size, int64_t stride_page,
+                                int64_t stride_head, int32_t *error_flag, void *stream);
+
 /* What the given slots stand for: k_out / v_out [tokens, hkv, head_dim], fp32 or bf16 (zeros for
  * slot -1). */
 int mrb_kv4_read(const void *pool, int64_t num_pages, int64_t hkv, int64_t head_dim, int64_t group,

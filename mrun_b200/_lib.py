@@ -100,6 +100,8 @@ SIGNATURES: dict[str, list] = {
     "mrb_kv_release": [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _P],
     "mrb_rope_kv4_append": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, c_int,
                             _P, _P, c_float, _P, _P, _I64, _I64, _I64, _I64, _P, _P],
+    "mrb_rope_kv4_append_strided": [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64,
+                                    _I64, c_int, _P, _P, c_float, _P, _P, _I64, _I64, _I64, _I64, _P, _P],
     "mrb_kv4_read": [_P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, c_int, _P, _P],
     "mrb_kv4_paged_attention_timeouts": [],
     "mrb_kv4_prefill_attention_timeouts": [],

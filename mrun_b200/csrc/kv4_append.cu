@@ -23,7 +23,7 @@ constexpr int KA_ITERS = 4;  // vectors a lane group takes in one go
 
 struct Kv4AppendArgs {
   const __nv_bfloat16 *q, *k, *v;
-  int64_t in_stride, v_stride;
+  int64_t q_stride, k_stride, v_stride;
   const int32_t *positions, *slots;
   const float *cos, *sin;
   const __nv_bfloat16 *q_norm, *k_norm;
@@ -125,7 +125,7 @@ __device__ __forceinline__ void append_queries(const Kv4AppendArgs& a, int64_t t
     const int h = first + i * PER;
     in[i][0] = in[i][1] = make_uint2(0u, 0u);
     if (h >= a.hq) continue;
-    const __nv_bfloat16* src = a.q + t * a.in_stride + (int64_t)h * D;
+    const __nv_bfloat16* src = a.q + t * a.q_stride + (int64_t)h * D;
     in[i][0] = __ldg(reinterpret_cast<const uint2*>(src + da));
     in[i][1] = __ldg(reinterpret_cast<const uint2*>(src + db));
   }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) rope_kv4_append_kernel(const __
     const int h = first + i * PER + sub;
     in[i] = make_uint2(0u, 0u);
     if (h >= heads) continue;
-    const __nv_bfloat16* src = h < a.hkv ? a.k + t * a.in_stride + (int64_t)h * D
+    const __nv_bfloat16* src = h < a.hkv ? a.k + t * a.k_stride + (int64_t)h * D
                                          : a.v + t * a.v_stride + (int64_t)(h - a.hkv) * D;
     in[i] = __ldg(reinterpret_cast<const uint2*>(src + d0));
   }
@@ -324,13 +324,14 @@ static int launch_read(const Kv4ReadArgs& a, int dtype, cudaStream_t s) {
 
 }  // namespace mrb
 
-extern "C" int mrb_rope_kv4_append(const void* q_in, const void* k_in, const void* v_in, int64_t in_row_stride,
-                                   int64_t v_row_stride, int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
-                                   int64_t group, const int32_t* positions, const int32_t* slots,
-                                   const float* rope_cos, const float* rope_sin, int64_t rope_len, int64_t rotary_dim,
-                                   int interleaved, const void* q_norm, const void* k_norm, float norm_eps,
-                                   void* q_out, void* pool, int64_t num_pages, int64_t page_size, int64_t stride_page,
-                                   int64_t stride_head, int32_t* error_flag, void* stream) {
+extern "C" int mrb_rope_kv4_append_strided(const void* q_in, const void* k_in, const void* v_in, int64_t q_row_stride,
+                                           int64_t k_row_stride, int64_t v_row_stride, int64_t tokens, int64_t hq,
+                                           int64_t hkv, int64_t head_dim, int64_t group, const int32_t* positions,
+                                           const int32_t* slots, const float* rope_cos, const float* rope_sin,
+                                           int64_t rope_len, int64_t rotary_dim, int interleaved, const void* q_norm,
+                                           const void* k_norm, float norm_eps, void* q_out, void* pool,
+                                           int64_t num_pages, int64_t page_size, int64_t stride_page,
+                                           int64_t stride_head, int32_t* error_flag, void* stream) {
   using namespace mrb;
   const char* what = "rope_kv4_append";
   Kv4AppendArgs a = {};
@@ -351,14 +352,15 @@ extern "C" int mrb_rope_kv4_append(const void* q_in, const void* k_in, const voi
   }
   if (!k_in || !v_in || !slots || (hq > 0 && (!q_in || !q_out)) || (rope_cos && !positions))
     return fail(MRB_ERR_ARG, "%s: null pointer", what);
-  if (!aligned(q_in, 8) || !aligned(k_in, 8) || !aligned(v_in, 8) || !aligned(q_out, 8) || in_row_stride % 4 ||
+  if (!aligned(q_in, 8) || !aligned(k_in, 8) || !aligned(v_in, 8) || !aligned(q_out, 8) || q_row_stride % 4 || k_row_stride % 4 ||
       v_row_stride % 4 || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || !aligned(q_norm, 8) ||
       !aligned(k_norm, 8))
     return fail(MRB_ERR_ARG, "%s: rows must be 8-byte aligned and rotary tables 16-byte aligned", what);
   a.q = (const __nv_bfloat16*)q_in;
   a.k = (const __nv_bfloat16*)k_in;
   a.v = (const __nv_bfloat16*)v_in;
-  a.in_stride = in_row_stride;
+  a.q_stride = q_row_stride;
+  a.k_stride = k_row_stride;
   a.v_stride = v_row_stride;
   a.positions = positions;
   a.slots = slots;
@@ -383,6 +385,19 @@ extern "C" int mrb_rope_kv4_append(const void* q_in, const void* k_in, const voi
   if (group == 32) return launch_append<128, 32>(a, interleaved, s);
   if (group == 64) return launch_append<128, 64>(a, interleaved, s);
   return launch_append<128, 128>(a, interleaved, s);
+}
+
+extern "C" int mrb_rope_kv4_append(const void* q_in, const void* k_in, const void* v_in, int64_t in_row_stride,
+                                   int64_t v_row_stride, int64_t tokens, int64_t hq, int64_t hkv, int64_t head_dim,
+                                   int64_t group, const int32_t* positions, const int32_t* slots,
+                                   const float* rope_cos, const float* rope_sin, int64_t rope_len, int64_t rotary_dim,
+                                   int interleaved, const void* q_norm, const void* k_norm, float norm_eps,
+                                   void* q_out, void* pool, int64_t num_pages, int64_t page_size, int64_t stride_page,
+                                   int64_t stride_head, int32_t* error_flag, void* stream) {
+  return mrb_rope_kv4_append_strided(q_in, k_in, v_in, in_row_stride, in_row_stride, v_row_stride, tokens, hq, hkv,
+                                     head_dim, group, positions, slots, rope_cos, rope_sin, rope_len, rotary_dim,
+                                     interleaved, q_norm, k_norm, norm_eps, q_out, pool, num_pages, page_size,
+                                     stride_page, stride_head, error_flag, stream);
 }
 
 extern "C" int mrb_kv4_read(const void* pool, int64_t num_pages, int64_t hkv, int64_t head_dim, int64_t group,

@@ -341,7 +341,6 @@ void rope_kv4_append(const std::optional<at::Tensor>& q_in, const at::Tensor& k_
                       ": q_in must hold whole heads of ", p.head_dim);
     hq = q_in->size(1) / p.head_dim;
     need_rows(*q_in, pool, t, hq * p.head_dim, "q_in", what);
-    TORCH_CHECK_VALUE(t <= 1 || q_in->stride(0) == k_in.stride(0), what, ": q_in and k_in must have one row stride");
     need(*q_out, at::kBFloat16, "q_out");
     need_same_device(*q_out, pool, what);
     TORCH_CHECK_VALUE(q_out->numel() == t * hq * p.head_dim, what, ": q_out must be [tokens, heads, head_dim]");
@@ -364,9 +363,11 @@ void rope_kv4_append(const std::optional<at::Tensor>& q_in, const at::Tensor& k_
       need_same_device(**w, pool, what);
       TORCH_CHECK_VALUE((*w)->numel() == p.head_dim, what, ": norm weights must be [head_dim]");
     }
+  const auto stride = [t](const at::Tensor& x) { return t > 1 ? x.stride(0) : 0; };  // of one row: not used
   check_status(
-      mrb_rope_kv4_append(has_q ? q_in->data_ptr() : nullptr, k_in.data_ptr(), v_in.data_ptr(), k_in.stride(0),
-                          v_in.stride(0), t, hq, p.hkv, p.head_dim, group, opt_i32(positions, pool, t, "positions", what),
+      mrb_rope_kv4_append_strided(
+                          has_q ? q_in->data_ptr() : nullptr, k_in.data_ptr(), v_in.data_ptr(),
+                          has_q ? stride(*q_in) : 0, stride(k_in), stride(v_in), t, hq, p.hkv, p.head_dim, group, opt_i32(positions, pool, t, "positions", what),
                           slots.data_ptr<int32_t>(), opt_ptr<float>(rope_cos), opt_ptr<float>(rope_sin),
                           rope ? rope_cos->size(0) : 0, rope ? 2 * rope_cos->size(1) : 0, interleaved ? 1 : 0,
                           opt_ptr<void>(q_norm), opt_ptr<void>(k_norm), (float)norm_eps, opt_ptr<void>(q_out),

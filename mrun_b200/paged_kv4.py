@@ -195,8 +195,8 @@ def rope_kv4_append(
     """Rotate queries and keys and write keys and values to their slots in 4 bits.
 
     ``k_in`` / ``v_in``: bf16 rows [tokens, kv_heads * head_dim], ``q_in``: [tokens, num_heads *
-    head_dim] (slices of one fused projection output are fine). ``rope`` = (cos, sin) fp32
-    [positions, rotary_dim / 2]: the first rotary_dim dimensions of each head turn, in pairs
+    head_dim], each with a row stride of its own (slices of one fused projection output are fine).
+    ``rope`` = (cos, sin) fp32 [positions, rotary_dim / 2]: the first rotary_dim dimensions of each head turn, in pairs
     (d, d + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1). ``qk_norm`` = (q weight, k weight):
     per-head RMSNorm before the rotation. A token with slot -1 is rotated but not stored. Returns
     the rotated queries, bf16 [tokens, num_heads, head_dim] (None without ``q_in``)."""

@@ -174,3 +174,29 @@ def test_queries_of_no_block_give_zeros(cuda):
         got = kv4_prefill_attention(q, c.pool[0], group=head_dim, block_table=c.block_table, q_starts=_i32([0], cuda),
                                     row_len=none)
         assert not got.any()
+
+
+@pytest.mark.parametrize("tokens", [1, 37])
+@pytest.mark.parametrize("head_dim,group,interleaved", [(64, 32, True), (128, 128, False)])
+def test_append_of_separate_projections(head_dim, group, interleaved, tokens, cuda):
+    """Queries, keys and values of one fused row, of three tensors, and of slices of wider ones."""
+    from mrun_b200.paged_kv4 import rope_kv4_append
+
+    rng = np.random.default_rng(head_dim)
+    hq, hkv = 7, 2
+    fused = _bf(rng.standard_normal((tokens, (hq + 2 * hkv) * head_dim)), cuda)
+    parts = fused.split([hq * head_dim, hkv * head_dim, hkv * head_dim], 1)
+    apart = [x.contiguous() for x in parts]
+    wide = [torch.cat([x, torch.zeros(tokens, 4 * (i + 1), dtype=x.dtype, device=cuda)], 1)[:, :x.shape[1]]
+            for i, x in enumerate(parts)]
+    cos, sin = (torch.randn(tokens, head_dim // 2, device=cuda) for _ in range(2))
+    at = _i32(list(range(tokens)), cuda)
+    results = []
+    for q, k, v in (parts, apart, wide, (apart[0], parts[1], wide[2])):
+        pool = torch.zeros(3, hkv, 1, ok.block_bytes(head_dim, group), dtype=torch.uint8, device=cuda)
+        out = rope_kv4_append(k, v, pool, group=group, head_dim=head_dim, slots=at, positions=at, q_in=q, num_heads=hq,
+                              rope=(cos, sin), interleaved=interleaved)
+        results.append((out, pool))
+    assert results[0][0].any() and results[0][1].any()
+    for out, pool in results[1:]:
+        assert torch.equal(out, results[0][0]) and torch.equal(pool, results[0][1])
