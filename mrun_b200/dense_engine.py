@@ -321,6 +321,7 @@ class DenseDecoder:
         self.row_seq = torch.arange(b, dtype=torch.int32, device=device)
         if self.kv_bits == 4:
             self.one_token = torch.ones(b, dtype=torch.int32, device=device)  # new tokens of a decode step
+            self.reserved = [0] * b  # tokens that each sequence was promised room for
         self.graph: torch.cuda.CUDAGraph | None = None
         self.graph_rows = 0
         self.launches_per_step = 0
@@ -466,16 +467,18 @@ class DenseDecoder:
         return int(self.kv.lengths[seq])
 
     def reserve(self, seq: int, tokens: int) -> None:
-        """Map the pages of a sequence's first ``tokens`` tokens (a 4-bit cache maps each step's own
-        and is asked here only whether they would all fit)."""
+        """Set the pages of a sequence's first ``tokens`` tokens aside until it is released. (A 4-bit
+        cache maps each step's own; the pages are kept from prefills and reservations of others, not
+        from decode steps of sequences without one.)"""
         if self.kv_bits == 16:
             self.kv.reserve(seq, tokens)
         else:
             self._room({seq: tokens - self.length(seq)})
+            self.reserved[seq] = max(self.reserved[seq], tokens)
 
     def _room(self, new: dict[int, int]) -> list[int]:
         """Committed tokens of the sequences of ``new``, once it is sure that the 4-bit cache takes
-        that many more of each."""
+        that many more of each next to what is reserved."""
         *lengths, free = torch.cat([self.kv.lengths, self.kv.free_count]).tolist()
         if any(lengths[s] + n > self.max_seq_len for s, n in new.items()):
             raise OverflowError("input block exceeds KV cache capacity")
@@ -483,7 +486,8 @@ class DenseDecoder:
         def pages(tokens: int) -> int:
             return (tokens + self.kv.page_size - 1) // self.kv.page_size
 
-        if sum(pages(lengths[s] + max(n, 0)) - pages(lengths[s]) for s, n in new.items()) > free:
+        claims = [max(n, r, n + new.get(s, 0)) for s, (n, r) in enumerate(zip(lengths, self.reserved))]
+        if sum(pages(c) - pages(n) for c, n in zip(claims, lengths)) > free:
             raise MemoryError("the paged KV pool is exhausted")
         return [lengths[s] for s in new]
 
@@ -498,6 +502,7 @@ class DenseDecoder:
             self.kv.release(seq)
         else:
             self.kv.release(torch.tensor([seq], dtype=torch.int32, device=self.device))
+            self.reserved[seq] = 0
 
     # ------------------------------------------------------------------ decode
 

@@ -82,3 +82,34 @@ def test_positions_that_cannot_be_rounded_up_are_refused(call):
     """2^31 - 16 tokens a row: their last step's end is past 32 bits."""
     pages = (2 ** 31 - 1) // 16
     assert call(_lib.load(), per=pages, stride=pages) == _lib.MRB_ERR_UNSUPPORTED
+
+
+def test_reservations_of_a_4_bit_cache_hold_together():
+    """Two sequences that were each promised room have it, against each other and against a prefill."""
+    from mrun_b200.dense_engine import DenseDecoder
+
+    dec = object.__new__(DenseDecoder)
+    dec.kv_bits, dec.max_batch, dec.max_seq_len, dec.device = 4, 3, 256, torch.device("cpu")
+    dec.kv = paged_kv4.PagedKV4Cache(num_layers=1, num_pages=6, kv_heads=1, head_dim=64, max_seqs=3,
+                                     max_pages_per_seq=4, device=dec.device, page_size=64)
+    dec.reserved = [0] * 3
+    dec.kv.lengths[:] = torch.tensor([70, 0, 64])  # 2 + 0 + 1 pages
+    dec.kv.free_count.fill_(3)
+    dec.reserve(0, 192)  # one more page, which later calls may not take
+    with pytest.raises(MemoryError):
+        dec.reserve(1, 129)
+    dec.reserve(1, 100)
+    dec.reserve(0, 150)  # less than it has
+    assert dec.reserved == [192, 100, 0]
+    with pytest.raises(MemoryError):
+        dec.reserve(2, 65)
+    with pytest.raises(MemoryError):
+        dec._room({2: 1})
+    assert dec._room({0: 122, 1: 128}) == [70, 0]  # within their own
+    with pytest.raises(MemoryError):
+        dec._room({0: 123})
+    with pytest.raises(OverflowError):
+        dec.reserve(1, 257)
+    dec.kv.release = lambda seqs: None
+    dec.release(1)
+    dec.reserve(2, 192)
