@@ -456,8 +456,9 @@ class DenseDecoder:
         normed = self._layers(n, plan.positions, step[1], plan.row_len, max(starts) + max(counts), last_only=True,
                               prefill=(seqs[0], starts[0]), plan=plan)
         last = normed.index_select(0, plan.q_starts[1:].long() - 1)
-        idx, _, _ = qrow_argmax(self.w.head.codes, self.w.head.scales, last, store_logits=False)
+        idx, value, _ = qrow_argmax(self.w.head.codes, self.w.head.scales, last, store_logits=False)
         self.next_ids.index_copy_(0, step[1].long(), idx)
+        self.next_val.index_copy_(0, step[1].long(), value)
         return idx
 
     # ------------------------------------------------------------------ sequences

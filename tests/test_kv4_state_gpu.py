@@ -200,3 +200,33 @@ def test_append_of_separate_projections(head_dim, group, interleaved, tokens, cu
     assert results[0][0].any() and results[0][1].any()
     for out, pool in results[1:]:
         assert torch.equal(out, results[0][0]) and torch.equal(pool, results[0][1])
+
+
+def test_prefill_leaves_the_values_of_its_tokens(cuda):
+    """next_val holds the logit of each prefilled sequence's next token, as with a bf16 cache."""
+    from mrun_b200.dense_qstore_cuda import qrow_argmax
+
+    cfg, dec = _dense(cuda)
+    ids = torch.arange(100) * 3 % cfg.vocab
+    dec.next_val.fill_(float("nan"))
+    tokens = dec.prefill_batch([1, 0], [ids[:30], ids[30:]])
+    last = dec.buf["normed"][[29, 99]]
+    _, value, logits = qrow_argmax(dec.w.head.codes, dec.w.head.scales, last)
+    assert torch.equal(dec.next_val[[1, 0]], value) and dec.next_val.isfinite().all()
+    assert torch.equal(dec.next_ids[[1, 0]], tokens)
+    dec.next_val.fill_(float("nan"))
+    dec.prefill(0, ids[:5])
+    assert dec.next_val[0].isfinite() and dec.next_val[1].isnan()
+
+
+def test_two_generations_share_a_small_pool(cuda):
+    """A reservation outlives its generation until the sequence is released."""
+    cfg, dec = _dense(cuda, num_pages=3)
+    ids = torch.arange(20) % cfg.vocab
+    dec.generate(ids, 60)  # 80 tokens reserved: 2 pages
+    dec.prefill(1, ids)
+    with pytest.raises(MemoryError):
+        dec.reserve(1, 65)
+    dec.release(0)
+    dec.reserve(1, 65)
+    dec.check_errors()
