@@ -253,19 +253,34 @@ __global__ void __launch_bounds__(KP_THREADS) kv_release_kernel(const int32_t* s
 }  // namespace mrb
 
 namespace mrb {
-// Clusters of more than eight CTAs are asked for, once a device.
-static bool plan_wide_clusters() {
-  static std::atomic<uint64_t> granted{0};
+// Whether a cluster of KP_MAX_CTAS CTAs, each with `smem` bytes, fits the current device as it is now
+// configured: more than eight have to be asked for, and a GPU may have fewer SMs together. Asked once for
+// a size that is larger than those that fit, or smaller than those that do not.
+static bool plan_wide_clusters(size_t smem) {
+  static std::atomic<int64_t> fits[64], fails[64];  // largest and smallest size + 1
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return false;
-  if (granted.load() >> dev & 1) return true;
-  if (cudaFuncSetAttribute((const void*)kv_plan_step_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return false;
-  }
-  granted.fetch_or(uint64_t(1) << dev);
-  return true;
+  const int64_t size = (int64_t)smem + 1, bad = fails[dev].load();
+  if (size <= fits[dev].load()) return true;
+  if (bad && size >= bad) return false;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(KP_MAX_CTAS);
+  cfg.blockDim = dim3(KP_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = KP_MAX_CTAS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  const bool ok = cudaFuncSetAttribute((const void*)kv_plan_step_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed,
+                                       1) == cudaSuccess &&
+                  cudaOccupancyMaxActiveClusters(&clusters, (const void*)kv_plan_step_kernel, &cfg) == cudaSuccess &&
+                  clusters > 0;
+  if (!ok) cudaGetLastError();
+  (ok ? fits : fails)[dev].store(size);
+  return ok;
 }
 }  // namespace mrb
 
@@ -319,7 +334,7 @@ extern "C" int mrb_kv_plan_step(const int32_t* new_tokens, const int32_t* row_se
   const int64_t want = (max_tokens + 4 * KP_THREADS - 1) / (4 * KP_THREADS);
   int ctas = 1;
   while (ctas < KP_MAX_CTAS && ctas < want) ctas *= 2;
-  if (ctas > 8 && !plan_wide_clusters()) ctas = 8;
+  if (ctas > 8 && !plan_wide_clusters(smem)) ctas = 8;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(KP_THREADS);

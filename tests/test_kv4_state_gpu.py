@@ -230,3 +230,39 @@ def test_two_generations_share_a_small_pool(cuda):
     dec.release(0)
     dec.reserve(1, 65)
     dec.check_errors()
+
+
+def test_the_largest_plan(cuda):
+    """As many requests and sequences as a step takes: the most shared memory that the clusters need."""
+    from mrun_b200.paged_kv4 import kv_plan_step
+
+    rows, seqs, page = 8192, 1 << 18, 16
+    rng = np.random.default_rng(8)
+    new = rng.integers(0, 12, rows)
+    order = rng.permutation(seqs)[:rows]
+    lengths = rng.integers(0, 2 * page, seqs)
+    have, need = -(-lengths[order] // page), -(-(lengths[order] + new) // page)
+    table = np.full((seqs, 4), -1, np.int32)
+    ids = rng.permutation(2 * seqs + int((need - have).sum())).astype(np.int32)
+    table[:, :2] = ids[:2 * seqs].reshape(seqs, 2)
+    table[np.arange(4) >= -(-lengths // page)[:, None]] = -1
+    free = ids[2 * seqs:]
+    tb = torch.from_numpy(table).to(cuda)
+    ln, fc = _i32(lengths.tolist(), cuda), _i32([len(free)], cuda)
+    flag = _i32([0], cuda)
+    p = kv_plan_step(_i32(new.tolist(), cuda), ln, tb, torch.from_numpy(free).to(cuda), fc, row_seq=_i32(order.tolist(), cuda),
+                     page_size=page, max_tokens=int(new.sum()), error_flag=flag)
+    assert flag.item() == 0 and fc.item() == 0
+    taken = 0
+    for r in range(rows):
+        for j in range(have[r], need[r]):
+            table[order[r], j] = free[len(free) - 1 - taken]
+            taken += 1
+    row = np.repeat(np.arange(rows), new)
+    pos = lengths[order][row] + np.arange(new.sum()) - (np.cumsum(new) - new)[row]
+    assert np.array_equal(tb.cpu().numpy(), table)
+    assert np.array_equal(p.positions.cpu().numpy(), pos)
+    assert np.array_equal(p.token_rows.cpu().numpy(), order[row])
+    assert np.array_equal(p.slots.cpu().numpy(), table[order[row], pos // page] * page + pos % page)
+    lengths[order] += new
+    assert np.array_equal(ln.cpu().numpy(), lengths)
