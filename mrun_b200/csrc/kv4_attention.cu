@@ -383,7 +383,8 @@ kv4_decode_kernel(const __grid_constant__ Kv4DecodeArgs a) {
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         if (t == 0) qsum[gr][nt * 8 + g] = sum * 0x1p-24f;
       }
-      if (t == 0 && warp == 0) qscale[nt * 8 + g] = a.scale2 * __int_as_float((127 - up) << 23) * 0x1p24f;
+      // (not zero, which a masked score would make a NaN of)
+      if (t == 0 && warp == 0) qscale[nt * 8 + g] = fmaxf(a.scale2 * __int_as_float((127 - up) << 23) * 0x1p24f, 0x1p-126f);
     }
     __syncthreads();  // and the last group's merge is over
     float cs[NT][2];
