@@ -7,9 +7,10 @@
 // and the factors go elsewhere -- 2^-24 into the softmax scale and the final division, 16 into
 // the queries (K) or the output dimension (V). Queries are scaled by a power of two to at most
 // 2^14, so that fp16 holds bf16 ones exactly. Weights p s are rounded to fp16 (11 bits), relative
-// to a running maximum of their own, which they may pass by 2^8 before the accumulators are
-// rescaled; from 2^-14 below it fp16 rounds them to multiples of 2^-24. Sums, maxima and the p m
-// term are fp32.
+// to a running maximum of their own, over all groups of dimensions, which goes to 2^7 and which they
+// may pass by 2^8 before the accumulators are rescaled; from 2^-21 below it fp16 rounds them to
+// multiples of 2^-31 of it, so groups whose scales lie 2^21 below another's lose their codes. Sums,
+// maxima and the p m term are fp32.
 //
 // Memory and the instructions that unpack it bound it (256 rows of 4096 tokens at most x 32/8 heads, 680
 // MB: 194 us, 3.5 TB/s, with 860 instructions a warp and unit, half of the issue slots used by three
@@ -43,6 +44,7 @@ constexpr int KD_MAX_ROWS = 512;   // rows a launch
 constexpr int KD_MAX_STAGES = 6;
 constexpr int KD_TILES = 2;  // tiles a unit: what a warp fetches, waits for and weighs in one go
 constexpr int KD_UNIT = KD_TILES * KV4_TILE;
+constexpr float KD_ROOM = 0x1p-7f;  // of fp16's range, kept for small weights: its largest are 2^15
 constexpr int KD_CHUNK = 64;       // parts of a group summed at a time
 constexpr int KD_COUNTERS = MRB_KV4_COUNTER_BYTES;  // of the workspace, one a CTA
 
@@ -462,7 +464,7 @@ kv4_decode_kernel(const __grid_constant__ Kv4DecodeArgs a) {
           uint32_t most = w[0];
 #pragma unroll
           for (int gr = 1; gr < NG; ++gr) most = max_bf16x2(most, w[gr]);
-          top[j][h] = low_half(most);
+          top[j][h] = low_half(most) * KD_ROOM;
         }
       bool in[KD_TILES][2];
 #pragma unroll

@@ -93,6 +93,17 @@ def test_ordinary_values(head_dim, group, n, cuda):
     _check(k, v, ok.bf16(rng.standard_normal((1, hq, head_dim)) * 1.5), group, cuda)
 
 
+@pytest.mark.parametrize("power", [10, 14, 18])
+@pytest.mark.parametrize("head_dim,group", [(64, 32), (128, 32), (128, 64)])
+def test_value_groups_of_unlike_sizes(head_dim, group, power, cuda):
+    """One group of dimensions whose values are 2^10 to 2^18 times as large as the others'."""
+    rng = np.random.default_rng(power + head_dim + group)
+    n, hq, hkv = 200, 8, 2
+    k, v = (ok.bf16(rng.standard_normal((n, hkv, head_dim))) for _ in range(2))
+    v[..., :group] *= 2.0 ** power
+    _check(k, v, ok.bf16(rng.standard_normal((1, hq, head_dim))), group, cuda)
+
+
 @pytest.mark.parametrize("scale", [1e-20, 1e-37, -1e-20, 0.0])
 @pytest.mark.parametrize("n", [5, 64, 77])
 def test_scales_that_vanish(scale, n, cuda):
