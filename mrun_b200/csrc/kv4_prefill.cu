@@ -14,8 +14,10 @@
 //
 // K and V are m + s c by one fp16 fused multiply-add a pair of codes, which a mask leaves as the
 // subnormal c 2^-24 (an odd nibble: 16 c 2^-24) with the factors taken into s. To stay inside fp16,
-// a tile of K is scaled by a power of two to at most 16, V likewise, by the tile or, where its
-// tokens' sizes differ by more than 2^6, token by token; scores, weights and row sums take the powers
+// a tile of K is scaled by a power of two to at most 16 2^-10, where fp16 ends 2^-18 below the largest
+// key; where its tokens' sizes differ by more than 2^6, codes are made whole numbers first and the tile is
+// scaled to at most 2^15. V is scaled by the tile or, where its tokens' sizes differ as much, token by
+// token; scores, weights and row sums take the powers
 // back exactly (a weight carries its token's power, so the running maximum M is that of score plus
 // power, and a token with huge values and no weight costs others no precision). Queries are scaled
 // to fp16 by a power of two a row. Weights are rounded to fp16 (11 bits); M moves only when a row's
@@ -875,6 +877,22 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
                        kf_fma2(y & 0x000f000fu, even, add), kf_fma2(y & 0x00f000f0u, odd, add));
       }
     };
+    // of a tile whose tokens are far apart: codes as whole numbers, so that the scales leave room, and the
+    // values scaled by up = 2^(11 - e), to 2^15 at most
+    auto fill_far = [&](unsigned char* tile, int p, const uint32_t (&w)[KW], uint32_t prm, float up) {
+      const float s = __uint_as_float(prm << 16) * up, m = __uint_as_float(prm & 0xffff0000u) * up;
+      const uint32_t mul = kf_half2(s, s), add = kf_half2(m, m);
+      const auto number = [](uint32_t x) {  // two codes: 1024 + c, less 1024
+        return kf_fma2((x & 0x000f000fu) | 0x64006400u, 0x3c003c00u, 0xe400e400u);
+      };
+#pragma unroll
+      for (int c = 0; c < KW; ++c) {
+        const uint32_t x = w[c];
+        *reinterpret_cast<uint4*>(tile + p * SPAN * 128 + place[c]) =
+            make_uint4(kf_fma2(number(x), mul, add), kf_fma2(number(x >> 4), mul, add),
+                       kf_fma2(number(x >> 8), mul, add), kf_fma2(number(x >> 12), mul, add));
+      }
+    };
     auto power_of = [](float most) { return max(-60, (int)(__float_as_uint(most) >> 23) - 127 - 3); };
     int walked = 0;
     bool more;
@@ -906,14 +924,19 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
             next = copy(j + 1);
             load_pages(j + 2);
           }
-          // ---- the tile's sizes; where V's are far apart or no numbers, each token's
-          float kmost = 0.f, vmost = 0.f, vleast = INFINITY, size[KF_PASSES];
+          // ---- the tile's sizes, and the smallest token's of K; where V's are far apart or no numbers, each
+          // token's
+          float kmost = 0.f, kleast = INFINITY, vmost = 0.f, vleast = INFINITY, size[KF_PASSES];
           bool plain = have == (1u << KF_PASSES) - 1u;
 #pragma unroll
           for (int p = 0; p < KF_PASSES; ++p) {
             const float ks = __uint_as_float(kp[p] << 16), km = __uint_as_float(kp[p] & 0xffff0000u);
-            const float kx = fmaxf(fabsf(km), fabsf(fmaf(15.f, ks, km)));
-            kmost = fmaxf(kmost, kx < 3e38f ? kx : 0.f);  // a NaN stays one, whatever the scale
+            float kx = fmaxf(fabsf(km), fabsf(fmaf(15.f, ks, km)));
+            kx = kx < 3e38f ? kx : 0.f;  // a NaN stays one, whatever the scale
+            if (NG > 1) kx = fmaxf(kx, __shfl_xor_sync(0xffffffffu, kx, 2));  // of the token's other groups
+            if (NG > 2) kx = fmaxf(kx, __shfl_xor_sync(0xffffffffu, kx, 1));
+            kmost = fmaxf(kmost, kx);
+            kleast = fminf(kleast, kx > 0.f ? kx : kleast);
             const float vs = __uint_as_float(vp[p] << 16), vm = __uint_as_float(vp[p] & 0xffff0000u);
             size[p] = kf_max_nan(fabsf(vm), fabsf(fmaf(15.f, vs, vm)));
             const float vx = size[p] < 3e38f ? size[p] : 0.f;
@@ -923,17 +946,20 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
           }
           // of numbers that are not negative, as their bits
           kmost = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(kmost)));
+          kleast = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(kleast)));
           vmost = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vmost)));
           vleast = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(plain ? vleast : 0.f)));
-          if (lane == 0) *reinterpret_cast<float4*>(sh.red[st][fw]) = make_float4(kmost, vmost, vleast, 0.f);
+          if (lane == 0) *reinterpret_cast<float4*>(sh.red[st][fw]) = make_float4(kmost, vmost, vleast, kleast);
           asm volatile("bar.sync 1, 256;" ::: "memory");
           const float4 other = *reinterpret_cast<const float4*>(sh.red[st][lane % (KF_FILL / 32)]);
           kmost = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(other.x)));
           vmost = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(other.y)));
           vleast = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(other.z)));
+          kleast = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(other.w)));
           const int ke = power_of(kmost), ve = power_of(vmost);
           const bool uniform = vleast > 0.f && vleast >= vmost * 0x1p-6f;  // (0: not every token is there)
-          const float k14 = kf_pow2(14 - ke), k10 = kf_pow2(-10 - ke), ve14 = kf_pow2(14 - ve), ve10 = kf_pow2(-10 - ve);
+          const bool far = kleast < kmost * 0x1p-6f;  // keys beside which others would lose bits
+          const float k14 = kf_pow2((far ? 11 : 14) - ke), k10 = kf_pow2(-10 - ke), ve14 = kf_pow2(14 - ve), ve10 = kf_pow2(-10 - ve);
           float v14[KF_PASSES], v10[KF_PASSES];
 #pragma unroll
           for (int p = 0; p < KF_PASSES; ++p) v14[p] = ve14, v10[p] = ve10;
@@ -963,7 +989,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
               for (int p = 0; p < KF_PASSES; ++p) sh.power[m][p * SPAN + tok0] = (float)ve;
           }
           if (ft == 0) {
-            sh.k_scale[m] = kf_pow2(ke);
+            sh.k_scale[m] = kf_pow2(far ? ke - 21 : ke);
             sh.v_power[m] = (float)ve;
             sh.v_undo[m] = kf_pow2(-ve);
             sh.uniform[m] = uniform;
@@ -973,7 +999,10 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
           if (walked >= 2) kf_wait(&sh.k_empty[st], ((walked >> 1) - 1) & 1, sh);
           __syncwarp();
 #pragma unroll
-          for (int p = 0; p < KF_PASSES; ++p) fill(sk + st * TILE_BYTES, p, kw[p], kp[p], k14, k10);
+          for (int p = 0; p < KF_PASSES; ++p) {
+            if (far) fill_far(sk + st * TILE_BYTES, p, kw[p], kp[p], k14);
+            else fill(sk + st * TILE_BYTES, p, kw[p], kp[p], k14, k10);
+          }
           fence_proxy_async_smem();
           mbar_arrive(&sh.k_full[st]);
           if (walked >= 2) kf_wait(&sh.v_empty[st], ((walked >> 1) - 1) & 1, sh);

@@ -93,6 +93,20 @@ def test_ordinary_values(head_dim, group, n, cuda):
     _check(k, v, ok.bf16(rng.standard_normal((1, hq, head_dim)) * 1.5), group, cuda)
 
 
+@pytest.mark.parametrize("power", [8, 14, 20])
+@pytest.mark.parametrize("head_dim,group", SHAPES)
+def test_a_key_far_above_its_neighbours(head_dim, group, power, cuda):
+    """A key 2^8 to 2^20 times as large as the others, which no query weighs: the others keep their bits."""
+    rng = np.random.default_rng(power + head_dim + group)
+    n, hq, hkv = 200, 8, 2
+    k, v = (ok.bf16(rng.standard_normal((n, hkv, head_dim))) for _ in range(2))
+    q = ok.bf16(rng.standard_normal((1, hq, head_dim)))
+    q[..., 0] = np.abs(q[..., 0]) + 2  # all queries share a direction, which the key is against
+    k[77] = 0
+    k[77, :, 0] = -2.0 ** power
+    _check(k, v, ok.bf16(q), group, cuda)
+
+
 @pytest.mark.parametrize("power", [10, 14, 18])
 @pytest.mark.parametrize("head_dim,group", [(64, 32), (128, 32), (128, 64)])
 def test_value_groups_of_unlike_sizes(head_dim, group, power, cuda):
