@@ -243,6 +243,7 @@ struct KfShared {
   int dead;  // a wait ran out: no later one waits
   KfPiece piece[KF_PIECES];
   int pieces, more, joins;
+  int rest;  // the first query of no block
   int cursor_row, cursor_tile, cursor_head;  // of the plan: where it goes on (row -1: not begun)
   int64_t cursor_at;
   KfCuts cuts;
@@ -292,6 +293,7 @@ __device__ __forceinline__ int64_t kf_length(const KfBlock& b, int span, int64_t
 __device__ __noinline__ void kf_plan(const Kv4PrefillArgs& a, KfShared& sh, int span, int lane) {
   const int hkv = a.pool.hkv, cta = blockIdx.x;
   if (sh.cursor_row < 0) {
+    if (lane == 0) sh.rest = max(0, a.q_starts[a.rows]);
     int64_t work = 0, tiles = 0;
     for (int r = lane; r < a.rows; r += 32) {
       const KfBlock b = kf_block(a, r, span);
@@ -520,6 +522,16 @@ __device__ __noinline__ void kf_place_queries(const Kv4PrefillArgs& a, KfShared&
   }
   fence_proxy_async_smem();
   mbar_arrive(&sh.q_full);
+}
+
+// Outputs of queries of no block, by the filling warps when their last tile is filled. (In the issuing
+// warpgroup, whose idle warps could write them at once, it cost the products' loop registers: nine ragged
+// blocks 343 us, and 337 so.)
+__device__ __noinline__ void kf_zero_rest(const Kv4PrefillArgs& a, int rest, int row) {
+  uint4* const out = reinterpret_cast<uint4*>(a.out);
+  const int64_t end = a.tokens * row, step = gridDim.x * KF_FILL;
+  for (int64_t x = (int64_t)rest * row + blockIdx.x * KF_FILL + threadIdx.x - KF_SOFTMAX; x < end; x += step)
+    out[x] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 template <int D, int G>
@@ -1013,6 +1025,7 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
           mbar_arrive(&sh.v_full[st]);
         }
       }
+      if (a.zero_rest && !more && sh.rest < a.tokens) kf_zero_rest(a, sh.rest, a.hq * (D / 8));
       kf_all_sync();
     } while (more);
   } else {
@@ -1037,18 +1050,10 @@ __global__ void __launch_bounds__(KF_THREADS, 1) kv4_prefill_kernel(const __grid
       if (i == 1) umma_commit(&sh.k_empty[at & 1]);
     };
     int walked = 0, turns = 0;
-    bool more, idle = warp != (KF_SOFTMAX + KF_FILL) / 32 && a.zero_rest;
+    bool more;
     do {
       kf_all_sync();
       more = sh.more;
-      if (idle) {  // the warps that issue nothing write the zeros
-        constexpr int FIRST = KF_SOFTMAX + KF_FILL + 32, COUNT = KF_THREADS - FIRST;
-        const int64_t row = (int64_t)a.hq * (D / 8), end = a.tokens * row;
-        const int from = max(0, a.q_starts[a.rows]);
-        for (int64_t x = from * row + blockIdx.x * COUNT + tid - FIRST; x < end; x += gridDim.x * COUNT)
-          reinterpret_cast<uint4*>(a.out)[x] = make_uint4(0u, 0u, 0u, 0u);
-        idle = false;
-      }
       const int pieces = warp == (KF_SOFTMAX + KF_FILL) / 32 ? sh.pieces : 0;
 #pragma unroll 1
       for (int n = 0; n < pieces; ++n) {
