@@ -69,13 +69,23 @@ def scaled_rope_tables(rotary_dim: int, theta: float, length: int, device: torch
       "original_max_position_embeddings"}``: long wavelengths divided by the factor, short ones
       kept, a linear blend between
     * ``{"rope_type": "yarn", "factor", "original_max_position_embeddings", "beta_fast",
-      "beta_slow", "attention_factor"}``: the same with a ramp over the dimensions, and both
-      tables times the attention factor (default 0.1 ln(factor) + 1)
+      "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"}``: the same with a ramp
+      over the dimensions (between whole ones unless ``truncate`` is false), and both tables times the
+      attention factor: by default 0.1 ln(factor) + 1, or with both ``mscale`` numbers
+      (0.1 mscale ln(factor) + 1) / (0.1 mscale_all_dim ln(factor) + 1)
     """
     if rotary_dim < 8 or rotary_dim % 8:
         raise ValueError("rotary_dim must be a positive multiple of 8")
     half = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    needs = {"default": (), "linear": ("factor",), "ntk": ("factor",),
+             "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+             "yarn": ("factor", "original_max_position_embeddings")}
+    if kind not in needs:
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    missing = [key for key in needs[kind] if scaling.get(key) is None] if needs[kind] else []
+    if missing:
+        raise ValueError(f"{kind} rotary scaling needs {', '.join(missing)}")
     factor = 1.0 if kind == "default" else float(scaling["factor"])
     if not math.isfinite(factor) or factor < 1.0:
         raise ValueError("a rotary scaling factor must be at least 1")
@@ -97,15 +107,21 @@ def scaled_rope_tables(rotary_dim: int, theta: float, length: int, device: torch
         def dim_of(turns: float) -> float:
             return rotary_dim * math.log(span / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        first = max(math.floor(dim_of(float(scaling.get("beta_fast") or 32))), 0)
-        last = min(math.ceil(dim_of(float(scaling.get("beta_slow") or 1))), rotary_dim - 1)
+        first, last = dim_of(float(scaling.get("beta_fast") or 32)), dim_of(float(scaling.get("beta_slow") or 1))
+        if scaling.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
         index = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
         keep = 1 - ((index - first) / max(last - first, 1e-3)).clamp(0, 1)
         inv = inv * keep + inv / factor * (1 - keep)
+
+        def magnitude(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0
+
         mult = scaling.get("attention_factor")
-        mult = 0.1 * math.log(factor) + 1.0 if mult is None else float(mult)
-    elif kind not in ("default", "ntk"):
-        raise ValueError(f"unknown rotary scaling {kind!r}")
+        if mult is None and scaling.get("mscale") and scaling.get("mscale_all_dim"):
+            mult = magnitude(float(scaling["mscale"])) / magnitude(float(scaling["mscale_all_dim"]))
+        mult = magnitude(1.0) if mult is None else float(mult)
     angle = torch.arange(length, dtype=torch.float64, device=device)[:, None] * inv
     return (angle.cos() * mult).float().contiguous(), (angle.sin() * mult).float().contiguous()
 

@@ -2,9 +2,11 @@
 capture and error bits."""
 from __future__ import annotations
 
+import math
 import re
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
@@ -113,3 +115,35 @@ def test_reservations_of_a_4_bit_cache_hold_together():
     dec.kv.release = lambda seqs: None
     dec.release(1)
     dec.reserve(2, 192)
+
+
+def test_yarn_tables_take_every_key():
+    """Published yarn configurations name a magnitude for all dimensions, and ramps between any two."""
+    base = {"rope_type": "yarn", "factor": 40.0, "original_max_position_embeddings": 4096}
+    cpu = torch.device("cpu")
+
+    def tables(**kw):
+        return [t.double().numpy() for t in paged_kv4.scaled_rope_tables(64, 1e4, 7, cpu, scaling=base | kw)]
+
+    plain = tables(attention_factor=1.0)
+    for kw, mult in (({}, 0.1 * math.log(40) + 1), ({"mscale": 1.0, "mscale_all_dim": 1.0}, 1.0),
+                     ({"mscale": 0.707, "mscale_all_dim": 1.0}, (0.0707 * math.log(40) + 1) / (0.1 * math.log(40) + 1)),
+                     ({"mscale": 0.707}, 0.1 * math.log(40) + 1),
+                     ({"attention_factor": 2.0, "mscale": 0.7, "mscale_all_dim": 1.0}, 2.0)):
+        for got, one in zip(tables(**kw), plain):
+            assert np.allclose(got, mult * one, rtol=2 ** -22, atol=2 ** -22)
+
+    def dim(turns):
+        return 64 * math.log(4096 / (turns * 2 * math.pi)) / (2 * math.log(1e4))
+
+    ramp = np.clip((np.arange(32) - dim(32)) / (dim(1) - dim(32)), 0, 1)
+    inv = 1e4 ** -(np.arange(0, 64, 2) / 64)
+    want = np.cos(np.arange(7)[:, None] * (inv * (1 - ramp) + inv / 40 * ramp))
+    assert np.allclose(tables(truncate=False, attention_factor=1.0)[0], want, atol=2 ** -22)
+
+
+@pytest.mark.parametrize("scaling", [{"rope_type": "spiral"}, {"rope_type": "linear"}, {"type": "yarn", "factor": 2.0},
+                                     {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0}])
+def test_rotary_scalings_that_are_not_whole_are_refused(scaling):
+    with pytest.raises(ValueError):
+        paged_kv4.scaled_rope_tables(16, 1e4, 4, torch.device("cpu"), scaling=scaling)
