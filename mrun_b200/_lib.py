@@ -268,20 +268,23 @@ class StreamScratch:
         index = device.index if device.index is not None else torch.cuda.current_device()
         # the raw handle: building a Stream object costs as much as the rest of a small call
         key = (index, torch._C._cuda_getCurrentRawStream(index))
-        capturing = torch.cuda.is_current_stream_capturing()
-        with self._lock:
-            buf = self._buffers.get(key)
-            have = buf is not None and buf.numel() >= nbytes
-            if not capturing:
-                if not have:
-                    buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
-                    self._buffers[key] = buf
-                return buf
+        buf = self._buffers.get(key)
+        have = buf is not None and buf.numel() >= nbytes
+        if not torch.cuda.is_current_stream_capturing():
+            return buf if have else self._grow(key, device, nbytes)
         if counters:
             buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
             buf[:counters].zero_()
             return buf
         return torch.zeros(nbytes, dtype=torch.uint8, device=device) if have else None
+
+    def _grow(self, key: tuple[int, int], device: torch.device, nbytes: int) -> torch.Tensor:
+        with self._lock:
+            buf = self._buffers.get(key)
+            if buf is None or buf.numel() < nbytes:
+                buf = torch.zeros(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=device)
+                self._buffers[key] = buf
+            return buf
 
 
 def exported_symbols() -> list[str]:
