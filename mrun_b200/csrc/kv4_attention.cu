@@ -12,11 +12,11 @@
 // multiples of 2^-31 of it, so groups whose scales lie 2^21 below another's lose their codes. Sums,
 // maxima and the p m term are fp32.
 //
-// Memory and the instructions that unpack it bound it (256 rows of 4096 tokens at most x 32/8 heads, 680
+// Memory and the instructions that unpack it bound it (calls in a row: 256 rows of 4096 tokens at most x 32/8 heads, 680
 // MB: 194 us, 3.5 TB/s, with 860 instructions a warp and unit, half of the issue slots used by three
-// warps a scheduler; copies of this size alone reach 6 TB/s) and, where the cache is short, latency (32
-// rows x 32/4 heads, 35 MB: 21 us; one row of 131071 tokens, 71 MB: 31 us: the first
-// loads of each warp and the join of the parts). A 16-token tile of one KV head is one contiguous block,
+// warps a scheduler, of 168 registers and 40 to 64 bytes spilled in the instances of <128, 32>; copies of
+// this size alone reach 6 TB/s) and, where the cache is short, latency (32 rows x 32/4 heads, 35 MB: 22 us;
+// one row of 131071 tokens, 71 MB: 31 us: the first loads of each warp and the join of the parts). A 16-token tile of one KV head is one contiguous block,
 // fetched by one bulk copy into the warp's ring. Tokens fill the 16 rows of mma.sync m16n8k16 and the group's
 // queries its 8 columns (NT of them): S^T = K Q^T, O^T += V^T P^T. A lane reads whole words of
 // codes: eight dimensions of a token are four register pairs of a K fragment (the order of
@@ -744,10 +744,10 @@ kv4_decode_kernel(const __grid_constant__ Kv4DecodeArgs a) {
 
 // Warps a CTA, twelve an SM in all (eight where two column blocks need more registers). Few groups,
 // of a long context, are each cut into many parts, whose sum is the last CTA's work: CTAs of a
-// whole SM leave the fewest (131071 tokens x 28/4 heads, a cold L2 and the launch with it: 37 us,
-// against 49 with four warps and 82 with two). Else small CTAs: a group's end then holds up few warps.
-// 32 rows of 256..4096 tokens x 32/4 heads: 29 us with four warps, 31 with two, 34 with twelve; 256
-// rows x 32/8 heads of 256 tokens: 51 us with two, 58 with four, 96 with twelve.
+// whole SM leave the fewest (131071 tokens x 28/4 heads: 37 us, against 49 with four warps and 82 with
+// two). Else small CTAs: a group's end then holds up few warps. 32 rows of 256..4096 tokens x 32/4 heads:
+// 29 us with four warps, 31 with two, 35 with twelve; 256 rows x 32/8 heads of 256 tokens: 45 us with two,
+// 49 with four, 78 with twelve. (Single calls, with a cold L2 and the launch: 7 us more than calls in a row.)
 static int kd_warps(int64_t rows, int64_t hkv, int nt) {
   const int64_t groups = rows * hkv;
   if (nt == 1 && groups >= 4 * num_sms()) return 2;

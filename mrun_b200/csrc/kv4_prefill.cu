@@ -28,8 +28,9 @@
 // as many as the products take at the tensor peak) and by shared memory (the products' operands and
 // the dequantised tiles: 2048 clocks a step). A step takes 4,000 clocks: the weights lie over the
 // scores, so a half's next scores wait for the product that reads its weights. 4096 tokens at 16384 x
-// 28/4 heads: 1.04 ms, 1040 TFLOP/s; 512 tokens alone: 29 us, of which 7 us are the plan and the first
-// loads, 4 us a tile's queries, and 5 us its first step.
+// 28/4 heads: 1.07 ms in single calls after a pause, 1010 TFLOP/s, and 1.16 one after another, under the
+// power limit; 512 tokens alone: 29 us, of which 7 us are the plan and the first loads, 4 us a tile's
+// queries, and 5 us its first step.
 #include "kv4.cuh"
 #include "qrow_common.cuh"
 #include "tc_common.cuh"
@@ -266,8 +267,8 @@ __device__ __forceinline__ void kf_all_sync() { asm volatile("bar.sync 0, 896;" 
 //
 // The work is measured in keys: a tile is as long as the keys that its last token sees, and KF_TILE_COST
 // more. All tiles in a line (by request, tile, head) are cut into equal shares, one a CTA, so that every
-// SM has as much to do whatever the blocks' lengths (4096 tokens at 16384, 456 tiles on 148 SMs:
-// 1.04 ms, and 1.25 with whole tiles only, where twelve of them made a last round; 64 tokens at 8000, 16
+// SM has as much to do whatever the blocks' lengths (4096 tokens at 16384, 456 tiles on 148 SMs: a
+// sixth less time than with whole tiles only, where twelve of them made a last round; 64 tokens at 8000, 16
 // tiles: 61 us against 155). A tile under a cut is divided at a step, or goes to one side as a whole if
 // the cut is within KF_LEAST steps of its ends.
 struct KfBlock {

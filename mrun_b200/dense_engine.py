@@ -288,7 +288,7 @@ class DenseDecoder:
         self.max_prefill_tokens = int(max_prefill_tokens)
         rows = max(self.max_batch, self.max_prefill_tokens)
         # the split plan depends on the row count: size for the worst row count we will run
-        attn_rows = rows if self.kv_bits == 16 else self.max_batch  # a 4-bit prefill takes none
+        attn_rows = rows if self.kv_bits == 16 else self.max_batch  # a 4-bit prefill takes its stream's own
         ws = max(self.kv.workspace_bytes(r, cfg.heads, self.max_seq_len) for r in range(1, attn_rows + 1))
         self.workspace = torch.zeros(max(ws, 256), dtype=torch.uint8, device=device)
         # GEMV stream-K workspace shared by every projection (all ordered on one stream)
