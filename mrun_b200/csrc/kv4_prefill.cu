@@ -22,7 +22,7 @@
 // power, and a token with huge values and no weight costs others no precision). Queries are scaled
 // to fp16 by a power of two a row. Weights are rounded to fp16 (11 bits); M moves only when a row's
 // weights of one step pass 2^13 together (so that no maximum is taken in most steps), and O is
-// rescaled in TMEM then.
+// rescaled in TMEM then. A weight 2^-25 below 2^M vanishes: n such tokens cost at most n 2^-25 of an output.
 //
 // Bound by the softmax's exponentials (16 a clock an SM: 2048 clocks a step of 256 rows x 128 keys,
 // as many as the products take at the tensor peak) and by shared memory (the products' operands and

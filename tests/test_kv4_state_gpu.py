@@ -266,3 +266,36 @@ def test_the_largest_plan(cuda):
     assert np.array_equal(p.slots.cpu().numpy(), table[order[row], pos // page] * page + pos % page)
     lengths[order] += new
     assert np.array_equal(ln.cpu().numpy(), lengths)
+
+
+def test_captured_projections_outlive_the_streams_workspace(cuda):
+    """The same of the default workspace that row-quantised projections split their tiles through."""
+    from mrun_b200.dense_qstore_cuda import qrow_linear
+
+    gen = torch.Generator(device=cuda).manual_seed(3)
+
+    def page(rows, k):
+        return (torch.randint(-127, 128, (rows, k), generator=gen, device=cuda, dtype=torch.int8),
+                torch.rand(rows, generator=gen, device=cuda) / 127)
+
+    x = torch.randn(1, 4096, generator=gen, device=cuda).to(torch.bfloat16)
+    small, large = page(3584, 4096), page(40000, 4096)
+    want = qrow_linear(*small, x)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        qrow_linear(*small, x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = qrow_linear(*small, x)
+    with torch.cuda.stream(side):
+        qrow_linear(*large, x)
+    torch.cuda.synchronize()
+    taken = [torch.full((1 << 20,), 255, dtype=torch.uint8, device=cuda) for _ in range(16)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert all((t == 255).all() for t in taken)
